@@ -43,6 +43,8 @@ UNITS = {
     "state_space": ["selective_scan.cu"],
     "token_input": ["token_input.cu"],
     "decay_state": ["decay_state.cu"],
+    "fp8": ["fp8_rows.cu", "linear_fp8.cu"],
+    "scores": ["token_logprobs.cu"],
 }
 
 

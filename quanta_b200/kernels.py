@@ -26,7 +26,7 @@ _STATUS_TEXT = {1: "token id outside the vocabulary", 2: "page id outside the po
                 7: "a position beyond the table of learned position vectors"}
 _KERNEL_TEXT = {1: "embedding", 2: "rope/cache write", 3: "paged attention", 4: "expert plan",
                 5: "expert product", 6: "decode attention", 7: "prefill attention", 8: "state slots",
-                9: "delta rule", 10: "router"}
+                9: "delta rule", 10: "router", 11: "e4m3 product", 12: "token scores"}
 
 
 class KernelError(RuntimeError):
@@ -1254,6 +1254,156 @@ def glu_act(gate_up: torch.Tensor, out: torch.Tensor, *, bias=None, kind: int = 
         raise ValueError("glu_act: the clamped form needs a positive limit")
     _check(lib().qb_glu_act(_p(gate_up), _code(gate_up), _p(bias), _p(out), _code(out), n, two_i // 2, int(kind),
                             ctypes.c_float(limit), ctypes.c_float(alpha), _stream()), "glu_act")
+
+
+FP8_BLOCK = 128                 # columns of a row, and rows and columns of a weight, that share a scale
+E4M3 = torch.float8_e4m3fn
+
+
+def _here(what: str, **tensors) -> None:
+    """All of them on the current device (the kernel is launched on its stream)."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+            raise ValueError(f"{what}: {name} is on {t.device}, which is not the current CUDA device")
+
+
+def _fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, cols: int, name: str) -> None:
+    _want(q, E4M3, name); _want(scales, torch.float32, f"the scales of {name}")
+    blocks = -(-cols // FP8_BLOCK)
+    if tuple(q.shape) != (n, cols) or tuple(scales.shape) != (blocks, n):
+        raise ValueError(f"{what}: {name} must be [{n}, {cols}] and its scales [{blocks}, {n}], got {tuple(q.shape)} and {tuple(scales.shape)}")
+
+
+def add_rmsnorm_fp8(h: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
+                    rows: torch.Tensor | None = None, store_h: bool = True, *, delta_gain: torch.Tensor | None = None,
+                    delta_eps: float = 0.0) -> None:
+    """``add_rmsnorm`` whose normed rows come out in e4m3, with a float32 scale for every row and 128 columns: ``out`` ``[n, H]``
+    float8_e4m3fn, ``scales`` ``[ceil(H / 128), n]``, the numbers they stand for ``out[r, c] * scales[c // 128, r]``.  A scale is the
+    block's largest number / 448, at least 2^-100 / 448.  ``delta`` (``[T, H]`` or ``[T, S, H]``, float32 or bfloat16, or None) is summed
+    over its slots; with ``delta_gain`` (float32 ``[H]``) it is normed first, ``delta_gain * d * rsqrt(mean(d^2) + delta_eps)``.
+    ``rows`` (int32) selects token rows, which needs ``store_h`` False (a row may be selected twice); one outside ``h`` gives NaN."""
+    _want(h, torch.float32, "h"); _want(weight, torch.float32, "weight")
+    if h.dim() != 2:
+        raise ValueError("add_rmsnorm_fp8: h must be [T, H]")
+    T, H = h.shape
+    S = 1
+    if delta is not None:
+        S = delta.shape[1] if delta.dim() == 3 else 1
+        if delta.dim() not in (2, 3) or delta.shape[0] != T or delta.shape[-1] != H or S < 1:
+            raise ValueError("add_rmsnorm_fp8: delta shape mismatch")
+    if delta_gain is not None:
+        _want(delta_gain, torch.float32, "delta_gain")
+        if delta is None or delta_gain.numel() != H:
+            raise ValueError("add_rmsnorm_fp8: delta_gain needs a delta and H numbers")
+    n = T if rows is None else rows.numel()
+    if rows is not None:
+        _want(rows, torch.int32, "rows")
+        if store_h and delta is not None:
+            raise ValueError("add_rmsnorm_fp8: selected rows are not stored back (store_h must be False)")
+    if weight.numel() != H:
+        raise ValueError("add_rmsnorm_fp8: weight shape mismatch")
+    _fp8_rows("add_rmsnorm_fp8", out, scales, n, H, "out")
+    _here("add_rmsnorm_fp8", h=h, delta=delta, weight=weight, delta_gain=delta_gain, out=out, scales=scales, rows=rows)
+    _check(lib().qb_add_rmsnorm_fp8(_p(h), _p(delta), _code(delta) if delta is not None else F32, S, _p(weight), _p(delta_gain), _p(out),
+                                    _p(scales), _p(rows), n, T, H, ctypes.c_float(eps), ctypes.c_float(delta_eps), int(store_h), _stream()),
+           "add_rmsnorm_fp8")
+
+
+def glu_act_fp8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, *, bias: torch.Tensor | None = None, kind: int = GLU_SILU,
+                limit: float = 0.0, alpha: float = 1.0) -> None:
+    """``glu_act`` whose result comes out in e4m3 with scales as those of ``add_rmsnorm_fp8``: ``gate_up`` ``[n, 2 I]`` float32 or bfloat16,
+    ``out`` ``[n, I]``, ``scales`` ``[ceil(I / 128), n]``.  Nothing is rounded between the activation and e4m3."""
+    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+        raise ValueError("glu_act_fp8: gate_up must be [n, 2 I]")
+    n, two_i = gate_up.shape
+    if bias is not None:
+        _want(bias, torch.float32, "bias")
+        if bias.numel() != two_i:
+            raise ValueError("glu_act_fp8: the bias has 2 I numbers")
+    if kind not in (GLU_SILU, GLU_CLAMPED, GLU_GELU_TANH):
+        raise ValueError(f"glu_act_fp8: no activation {kind}")
+    if kind == GLU_CLAMPED and not limit > 0:
+        raise ValueError("glu_act_fp8: the clamped form needs a positive limit")
+    _fp8_rows("glu_act_fp8", out, scales, n, two_i // 2, "out")
+    _here("glu_act_fp8", gate_up=gate_up, bias=bias, out=out, scales=scales)
+    _check(lib().qb_act_fp8(_p(gate_up), _code(gate_up), _p(bias), _p(out), _p(scales), n, two_i // 2, int(kind), ctypes.c_float(limit),
+                            ctypes.c_float(alpha), _stream()), "glu_act_fp8")
+
+
+def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
+    """Rows ``x`` ``[n, K]`` (float32 or bfloat16) in e4m3, with scales as those of ``add_rmsnorm_fp8``."""
+    if x.dim() != 2:
+        raise ValueError("rows_to_fp8: x must be [n, K]")
+    n, K = x.shape
+    _fp8_rows("rows_to_fp8", out, scales, n, K, "out")
+    _here("rows_to_fp8", x=x, out=out, scales=scales)
+    _check(lib().qb_act_fp8(_p(x), _code(x), _p(None), _p(out), _p(scales), n, K, 3, ctypes.c_float(0.0), ctypes.c_float(1.0), _stream()),
+           "rows_to_fp8")
+
+
+def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+               status: torch.Tensor | None = None) -> None:
+    """``out [T, N] = x [T, K] @ w [N, K].T`` of e4m3 matrices, ``x`` with scales ``[ceil(K / 128), T]`` (``add_rmsnorm_fp8``), ``w`` with a
+    scale for every block of 128 x 128, ``[ceil(N / 128), ceil(K / 128)]``.  A block's products are summed by the tensor cores, the blocks
+    scaled and summed in float32; ``out`` float32 or bfloat16 (one rounding).  K a multiple of 16; ``x`` and ``w`` on 16 bytes.  The same
+    operands give the same bits in every run.  ``status``: where a bounded wait that ran out is recorded (the outputs are NaN then)."""
+    _want(w, E4M3, "w"); _want(w_scales, torch.float32, "w_scales")
+    if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
+        raise ValueError("linear_fp8: x, w and out must be matrices")
+    T, K = x.shape
+    N = w.shape[0]
+    _fp8_rows("linear_fp8", x, x_scales, T, K, "x")
+    if w.shape[1] != K or tuple(out.shape) != (T, N):
+        raise ValueError(f"linear_fp8: w {tuple(w.shape)} and out {tuple(out.shape)} do not fit x {tuple(x.shape)}")
+    if tuple(w_scales.shape) != (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK)):
+        raise ValueError(f"linear_fp8: w_scales must be [{-(-N // FP8_BLOCK)}, {-(-K // FP8_BLOCK)}], got {tuple(w_scales.shape)}")
+    if K == 0 or K % 16:
+        raise ValueError(f"linear_fp8: K must be a positive multiple of 16, got {K}")
+    if status is not None:
+        _want(status, torch.int32, "status")
+    _here("linear_fp8", x=x, x_scales=x_scales, w=w, w_scales=w_scales, out=out, status=status)
+    _check(lib().qb_linear_fp8(_p(x), _p(x_scales), _p(w), _p(w_scales), _p(out), _code(out), T, K, N, _p(status), _stream()), "linear_fp8")
+
+
+TOKEN_LOGPROBS_MAX_TOP = 64
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: torch.Tensor | None, entropy: torch.Tensor | None,
+                   ids: torch.Tensor | None = None, best: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Of every row of ``logits`` ``[n, V]`` (float32 or bfloat16, rows of any stride): ``logprob`` (float32 ``[n]``), the log probability of
+    the row's token in ``tokens`` (int32 ``[n]``); ``entropy`` (float32 ``[n]``, in nats); ``ids`` (int32 ``[n, k]``) and ``best`` (float32 ``[n, k]``),
+    the k <= ``TOKEN_LOGPROBS_MAX_TOP`` most probable tokens, most probable first, equal ones by their id, and their log probabilities.  What
+    is None is not wanted.  A logit of -inf is a token of probability zero.  A row with a NaN or +inf, or with nothing but -inf, has NaN for
+    all numbers, and its tokens in the order of the logits with NaN as -inf.  A token outside the vocabulary is recorded in ``status``; its
+    log probability is NaN."""
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise ValueError("token_logprobs: logits must be [n, V] with rows of neighbouring numbers")
+    n, V = logits.shape
+    if V == 0:
+        raise ValueError("token_logprobs: an empty vocabulary")
+    if (logprob is None) != (tokens is None):
+        raise ValueError("token_logprobs: logprob and tokens belong together")
+    if (ids is None) != (best is None):
+        raise ValueError("token_logprobs: ids and best belong together")
+    for t, name, dtype in ((tokens, "tokens", torch.int32), (logprob, "logprob", torch.float32), (entropy, "entropy", torch.float32)):
+        if t is not None:
+            _want(t, dtype, name)
+            if tuple(t.shape) != (n,):
+                raise ValueError(f"token_logprobs: {name} must be [{n}], got {tuple(t.shape)}")
+    top = 0
+    if ids is not None:
+        _want(ids, torch.int32, "ids"); _want(best, torch.float32, "best")
+        top = ids.shape[1] if ids.dim() == 2 else -1
+        if top < 0 or tuple(ids.shape) != (n, top) or ids.shape != best.shape:
+            raise ValueError("token_logprobs: ids and best must be [n, k]")
+        if top > min(V, TOKEN_LOGPROBS_MAX_TOP):
+            raise ValueError(f"token_logprobs: {top} tokens a row of {V}; at most {TOKEN_LOGPROBS_MAX_TOP} are taken, and no more than there are")
+    if status is not None:
+        _want(status, torch.int32, "status")
+    _here("token_logprobs", logits=logits, tokens=tokens, logprob=logprob, entropy=entropy, ids=ids, best=best, status=status)
+    _check(lib().qb_token_logprobs(ctypes.c_void_p(logits.data_ptr()), _code(logits), ctypes.c_longlong(logits.stride(0)), _p(tokens), _p(logprob),
+                                   _p(entropy), _p(ids if top else None), _p(best if top else None), n, V, top, _p(status), _stream()),
+           "token_logprobs")
 
 
 def split2_bf16(x) -> torch.Tensor:
