@@ -2,18 +2,19 @@
 // of a row of x and for every 128 x 128 block of w, on the 5th-generation tensor cores.
 //
 // The scales change every 128 k, so what the tensor cores sum over one block of k is taken out of TMEM, scaled and added in float32 registers
-// (one rounding a block); two accumulators take turns, so that the tensor cores work on the next block meanwhile.  The weights are the
-// 128-row operand and the tokens the N operand: a block of 128 weight rows has one scale per k block, a token's scale belongs to a column, and a
-// step of few tokens still uses the full height of the MMA and reads its weights once.  A thread of the adding warps owns one weight row (a
-// TMEM lane) and up to 128 tokens.
+// (one rounding a block); two accumulators take turns, so that the tensor cores work on the next block meanwhile.  That addition has as
+// many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the two forms:
 //
-//   warp 0     : TMA producer: per k block the weight tile [128 x 128] and the token tile [NT x 128], 128-byte swizzle, into a ring of stages
-//   warp 1     : MMA issuer: 4 x tcgen05.mma (32 k each) a stage; commits free the stage and hand the accumulator over
-//   warp 2     : scales: xs[b, t] * ws[n / 128, b] of the tile's tokens into a ring in shared memory, fetched several blocks ahead
-//   warps 4-...: one TMEM lane quadrant each (two warps a quadrant where a tile has 128 tokens or more): add, then store
+//  * up to 64 tokens (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
+//    height of the MMA and the weights are read once.  A TMEM lane is a weight row, a column a token; the columns' scales come from shared memory.
+//  * more (linear_fp8_kernel): the tokens are the rows, the weights the columns.  A lane has its token's scale in a register and one weight
+//    scale for all of its columns, so the addition is one packed multiply-add for two numbers and reads nothing.  (With the tokens as columns the
+//    scales' way from shared memory to the registers, 128 KB a k block of 256 tokens, took 1,024 cycles: 8,192 x 4,096 x 22,016 1,175 us.)
+//    Steps of many tokens: two blocks on neighbouring SMs take 256 tokens x 256 weight rows together (cta_group::2), each fetching its own 128
+//    tokens and half of the weight tile.
 //
-// A matrix of few tiles is cut along k over the blocks of a cluster; each leaves its sums in shared memory, and every block adds one share of the
-// columns, the blocks' parts in order, so the result is the same in every run.
+// A product of few tiles is cut along k over the blocks of a cluster; each leaves its sums in shared memory, and every block adds one share of
+// them, the blocks' parts in order, so the result is the same in every run.
 //
 // Every wait on an mbarrier is bounded; when one runs out the block records it in the status words, its outputs are NaN, it lets its copies in
 // flight land, frees its TMEM and returns.
@@ -25,7 +26,8 @@ namespace {
 constexpr int L8_M = 128, L8_BK = 128;      // weight rows of a tile; k of a stage: 128 bytes, one swizzle row
 constexpr int L8_A = L8_M * L8_BK;          // bytes of a weight tile
 constexpr int L8_MAX_STAGES = 12, L8_SCALES = 4, L8_AHEAD = 3;      // slots of the scales' ring, blocks they are fetched ahead of it
-constexpr int L8_FIRST = 4;                 // the first adding warp (a warpgroup of its own: it has other numbers of registers)
+constexpr int L8_FIRST = 4;                 // the first adding warp
+constexpr int L8_FEW_THREADS = 256, L8_THREADS = 384;
 
 struct LinearFp8 {
   const float *xs, *ws;
@@ -57,19 +59,48 @@ __device__ __forceinline__ float l8_remote(uint32_t addr) {
   return v;
 }
 
-constexpr int l8_adders(int NT) { return NT >= 128 ? 8 : 4; }
-constexpr int l8_threads(int NT) { return (L8_FIRST + l8_adders(NT)) * 32; }
-// Tiles of 256 tokens: the adding threads hold 128 sums each, more registers than a block of 384 threads can give every one of them, so
-// the other warps hand some of theirs over.  What all have afterwards is what the block was launched with, at most.
-constexpr int L8_REGS_ADD = 216, L8_REGS_OTHER = 56, L8_REGS_LAUNCH = 168;
-static_assert(256 * L8_REGS_ADD + 128 * L8_REGS_OTHER <= 384 * L8_REGS_LAUNCH, "registers of the launch");
+constexpr int L8_NONE = 0x7fffffff;         // a NaN's bits
 
+// Eight parts of four neighbours, from the blocks of the cluster at this address, added in the order of the blocks.
+__device__ __forceinline__ float4 l8_sum_parts(uint32_t at, int cut) {
+  float4 v[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < cut)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w) : "r"(mapa_u32(at, (uint32_t)r)) : "memory");
+  }
+  float4 s = v[0];
+#pragma unroll
+  for (int r = 1; r < 8; ++r)
+    if (r < cut) s = make_float4(s.x + v[r].x, s.y + v[r].y, s.z + v[r].z, s.w + v[r].w);
+  return s;
+}
+// whether a block of the cluster gave up
+__device__ __forceinline__ bool l8_missing(int* flag, int cut) {
+  int missing = 0;
+  for (int r = 0; r < cut; ++r) missing |= __float_as_int(l8_remote(mapa_u32(smem_u32(flag), (uint32_t)r)));
+  return missing != 0;
+}
+template <typename O>
+__device__ __forceinline__ void l8_store4(O* row, int n, int N, float4 v) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < N) row[n + i] = qb_from_float<O>(f[i]);
+}
+
+//   warp 0     : TMA producer: per k block the weight tile [128 x 128] and the token tile [NT x 128], 128-byte swizzle, into a ring of stages
+//   warp 1     : MMA issuer: 4 x tcgen05.mma (32 k each) a stage; commits free the stage and hand the accumulator over
+//   warp 2     : scales: xs[b, t] * ws[n / 128, b] of the tile's tokens into a ring in shared memory, fetched several blocks ahead
+//   warps 4-7  : one TMEM lane quadrant each: add, then store
 // NT: tokens of a tile (the MMA's N)
 template <int NT, typename O>
-__global__ void __launch_bounds__(l8_threads(NT))
-linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, LinearFp8 a) {
+__global__ void __launch_bounds__(L8_FEW_THREADS)
+linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, LinearFp8 a) {
   qb_follow();
-  constexpr int ADDERS = l8_adders(NT), COLS = NT / (ADDERS / 4);      // columns an adding warp owns
+  constexpr int ADDERS = 4, COLS = NT;
   constexpr uint32_t STAGE = L8_A + NT * L8_BK;
   constexpr uint32_t TMEM = 2 * NT < 32 ? 32 : 2 * NT;
   extern __shared__ unsigned char smem_dyn[];
@@ -109,9 +140,6 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 
   O* out = reinterpret_cast<O*>(a.out);
 
-  if (warp < L8_FIRST) {
-    if constexpr (NT == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L8_REGS_OTHER));
-  }
   if (warp == 0) {
     if (lane == 0) {
       // weights that one token tile reads leave L2 first; tokens, and weights that others read too, stay
@@ -190,12 +218,11 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       }
     }
   } else if (warp >= L8_FIRST) {
-    if constexpr (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L8_REGS_ADD));
     float2 acc[COLS / 2];
   #pragma unroll
     for (int i = 0; i < COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-    const int quad = warp & 3, col0 = (warp - L8_FIRST) / 4 * COLS;
-    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)col0;
+    const int quad = warp & 3;
+    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16);
     bool ok = true;
 #pragma unroll 1
     for (int kb = 0; kb < k_blocks; ++kb) {
@@ -213,7 +240,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (c + 16 < COLS) tmem_ld16(from + (uint32_t)(half * NT + c + 16), v[(c / 16 + 1) & 1]);
         const uint32_t(&u)[16] = v[(c / 16) & 1];
-        const float4* sc = reinterpret_cast<const float4*>(&scales[slot][col0 + c]);
+        const float4* sc = reinterpret_cast<const float4*>(&scales[slot][c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 f = sc[i];
@@ -231,32 +258,30 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     if (a.cut == 1) {
       const int n = n0 + quad * 32 + lane;
       if (n < a.N) {
-        O* dst = out + (size_t)(t0 + col0) * a.N + n;
+        O* dst = out + (size_t)t0 * a.N + n;
 #pragma unroll
         for (int i = 0; i < COLS; ++i)
-          if (t0 + col0 + i < a.T) dst[(size_t)i * a.N] = qb_from_float<O>(!ok ? __int_as_float(0x7fffffff) : i & 1 ? acc[i / 2].y : acc[i / 2].x);
+          if (t0 + i < a.T) dst[(size_t)i * a.N] = qb_from_float<O>(!ok ? __int_as_float(L8_NONE) : i & 1 ? acc[i / 2].y : acc[i / 2].x);
       }
     } else if (ok) {
       // all products are done, so the ring is free: this block's sums [NT][128]
       float* part = reinterpret_cast<float*>(tiles);
 #pragma unroll
-      for (int i = 0; i < COLS; ++i) part[(col0 + i) * L8_M + quad * 32 + lane] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+      for (int i = 0; i < COLS; ++i) part[i * L8_M + quad * 32 + lane] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (a.cut > 1) {
     cluster_sync_all();
-    // a share of the columns, the blocks' parts in order; without the parts of a block that gave up it is no number
-    int missing = 0;
-    for (int r = 0; r < a.cut; ++r) missing |= __float_as_int(l8_remote(mapa_u32(smem_u32(&sh.abort_flag), (uint32_t)r)));
+    // a share of the columns; without the parts of a block that gave up it is no number
+    const bool missing = l8_missing(&sh.abort_flag, a.cut);
     const uint32_t part = smem_u32(tiles);
     const int share = (NT + a.cut - 1) / a.cut, c_end = min(min(NT, (rank + 1) * share), a.T - t0);
-    for (int i = rank * share * L8_M + (int)threadIdx.x; i < c_end * L8_M; i += blockDim.x) {
-      float sum = 0.f;
-      for (int r = 0; r < a.cut; ++r) sum += l8_remote(mapa_u32(part + 4u * i, (uint32_t)r));
-      const int n = n0 + i % L8_M;
-      if (n < a.N) out[(size_t)(t0 + i / L8_M) * a.N + n] = qb_from_float<O>(missing ? __int_as_float(0x7fffffff) : sum);
+    for (int i = rank * share * L8_M + (int)threadIdx.x * 4; i < c_end * L8_M; i += blockDim.x * 4) {
+      float4 sum = l8_sum_parts(part + 4u * i, a.cut);
+      if (missing) sum.x = sum.y = sum.z = sum.w = __int_as_float(L8_NONE);
+      l8_store4(out + (size_t)(t0 + i / L8_M) * a.N, n0 + i % L8_M, a.N, sum);
     }
     cluster_sync_all();      // the parts stay until all have read them
   }
@@ -264,40 +289,372 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   if (threadIdx.x == 0 && sh.abort_flag) qb_set_status(a.status, QB_STATUS_WAIT_TIMEOUT, tile, 11);
 }
 
-// [rows, K] e4m3, boxes of [box_rows, 128]
-int map_e4m3(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows) {
-  const cuuint64_t dims[2] = {K, rows}, strides[1] = {K};
-  const cuuint32_t box[2] = {L8_BK, box_rows};
-  return make_map(map, base, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+// ---------------------------------------------------------------------------------------------
+// More tokens.  A tile is 128 tokens x 128 weight rows, or, for a PAIR of blocks, 256 x 256, of which each block fetches its own 128 tokens and
+// half of the weights and holds the sums of its own tokens.
+//   warp 0     : TMA producer
+//   warps 1, 2 : MMA issuers (of a pair's first block), 4 x tcgen05.mma a job, N = 128.  A pair's k block is two jobs, the weight rows' halves, with
+//                accumulators of their own (four in all), so that the addition of one half runs under the products of the other.  An MMA is
+//                taken when the tensor cores are ready for it, and the waits and commits of a k block cost an issuer some 400 cycles besides the
+//                512 of its products, so two take the k blocks in turn.  (One issuer, N = 256, two accumulators: 984 cycles a k block, of which
+//                the tensor cores worked 512.)  The number of stages is even, so that a stage and an accumulator belong to one issuer, which
+//                waits for every phase of their barriers in order.
+//   warps 4-11 : a TMEM lane quadrant and 64 columns (a pair: 128) each: add, then store.  They hold up to 128 sums a thread, more registers than
+//                a block of 384 threads can give every one, so the other warps hand some of theirs over; what all have then is at most
+//                what the block was launched with.
+// Pairs walk over the tiles (a block an SM), so that the copies of the next tile run under the stores of the last; a block of a cut product has one.
+// Tiles go by groups of L8_GROUP token tiles, whose tokens and the weights that pass meanwhile stay in L2.
+constexpr int L8_REGS_ADD = 224, L8_REGS_OTHER = 56, L8_REGS_LAUNCH = 168, L8_GROUP = 8;
+static_assert(256 * L8_REGS_ADD + 128 * L8_REGS_OTHER <= L8_THREADS * L8_REGS_LAUNCH, "registers of the launch");
+constexpr int L8_BOX = 32 * 128;            // bytes of a warp's staged part of the output: 32 rows of 128 bytes
+constexpr uint32_t L8_STAGE = 2 * L8_A;     // 128 tokens and 128 weight rows
+
+struct L8Big {
+  uint64_t full[8], empty[8], acc_full[2][2], acc_empty[2][2];      // [half][turn]
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ void l8_arrive_at(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+__device__ __forceinline__ void l8_store_box(const CUtensorMap* map, uint32_t from, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(from) : "memory");
 }
 
-template <int NT, typename O>
-int l8_launch(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const LinearFp8& a, unsigned grid, size_t smem, cudaStream_t stream) {
-  auto kern = linear_fp8_kernel<NT, O>;
+template <bool PAIR, typename O>
+__global__ void __launch_bounds__(L8_THREADS, 1)
+linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
+                  LinearFp8 a, int boxes) {
+  qb_follow();
+  constexpr int SIDE = PAIR ? 256 : 128, HALVES = PAIR ? 2 : 1, COLS = PAIR ? 128 : 64;
+  constexpr uint32_t TMEM = HALVES * 256;
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  __shared__ L8Big sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR || a.cut > 1 ? (int)cluster_ctarank() : 0, width = PAIR ? 2 : a.cut;      // blocks of the cluster
+  const int k_first = PAIR ? 0 : rank * a.per, k_blocks = max(0, min(a.per, a.blocks - k_first));
+  const int n_tiles = (a.N + SIDE - 1) / SIDE, tiles_all = n_tiles * a.t_tiles;
+  const int tile_first = blockIdx.x / width, tile_step = gridDim.x / width;
+  volatile int* abort_flag = &sh.abort_flag;
+  // a tile's first weight row and this block's first token
+  auto place = [&](int tile, int& n0, int& t0) {
+    const int per_group = L8_GROUP * n_tiles, group = tile / per_group, in = tile - group * per_group;
+    const int high = min(L8_GROUP, a.t_tiles - group * L8_GROUP);
+    n0 = in / high * SIDE;
+    t0 = (group * L8_GROUP + in % high) * SIDE + (PAIR ? rank * 128 : 0);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(smem_u32(&sh.full[s]), 1);
+      mbar_init(smem_u32(&sh.empty[s]), 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(smem_u32(&sh.acc_full[s >> 1][s & 1]), 1);
+      mbar_init(smem_u32(&sh.acc_empty[s >> 1][s & 1]), 8);      // the warps that add: a half's four of each block of a pair
+    }
+    sh.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (PAIR) cluster_sync_all();      // both blocks' barriers exist before either counts on the other's
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = sh.tmem_base;
+  O* out = reinterpret_cast<O*>(a.out);
+
+  if (warp < L8_FIRST) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L8_REGS_OTHER));
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = l2_policy_evict_last();
+      const uint32_t full0 = smem_u32(&sh.full[0]), bars = PAIR ? mapa_u32(full0, 0u) : full0;
+      uint32_t parity = 1u;
+      int s = 0, armed = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int tile = tile_first; tile < tiles_all && ok; tile += tile_step) {
+        int n0, t0;
+        place(tile, n0, t0);
+        if (PAIR) n0 += rank * 128;
+#pragma unroll 1
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = mbar_wait(smem_u32(&sh.empty[s]), parity, abort_flag);
+          if (!ok) break;
+          const uint32_t st = smem_u32(tiles) + (uint32_t)s * L8_STAGE;
+          // (a pair: every copy of either block counts on the first block's barrier, which expects both blocks' bytes)
+          if (rank == 0 || !PAIR) mbar_expect_tx(full0 + 8u * s, HALVES * L8_STAGE);
+          if constexpr (PAIR) {
+            tma_load_2d_pair(st, &tm_x, kb * L8_BK, t0, bars + 8u * s, pol);
+            tma_load_2d_pair(st + L8_A, &tm_w, kb * L8_BK, n0, bars + 8u * s, pol);
+          } else {
+            tma_load_2d(st, &tm_x, (k_first + kb) * L8_BK, t0, full0 + 8u * s, pol);
+            tma_load_2d(st + L8_A, &tm_w, (k_first + kb) * L8_BK, n0, full0 + 8u * s, pol);
+          }
+          ++armed;
+          if (++s == a.stages) { s = 0; parity ^= 1u; }
+        }
+      }
+      if (*abort_flag && PAIR && rank != 0) {
+        // this block's copies count on the other block's barriers, which it cannot wait on: give them time
+        const uint64_t since = global_ns();
+        for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
+      } else if (*abort_flag) {
+        // let the copies that were issued land before this block's shared memory is given away
+        for (int i = max(0, armed - a.stages); i < armed; ++i) {
+          const uint64_t since = global_ns();
+          for (uint32_t it = 0; it < TC_SPIN_LIMIT && !mbar_try_wait(full0 + 8u * (i % a.stages), (uint32_t)(i / a.stages) & 1u); ++it)
+            if ((it & 63u) == 63u && global_ns() - since > TC_WAIT_NS) break;
+        }
+      }
+    }
+  } else if (warp < 3) {
+    if (lane == 0 && (rank == 0 || !PAIR)) {
+      const uint32_t idesc = umma_idesc_e4m3(PAIR ? 256 : 128, 128), buf = (uint32_t)warp - 1u;
+      const uint64_t a_first = umma_desc_sw128(smem_u32(tiles)), b_first = umma_desc_sw128(smem_u32(tiles) + L8_A);
+      const int mine = tile_first < tiles_all ? (tiles_all - tile_first + tile_step - 1) / tile_step : 0;
+      const int turns = mine * k_blocks;
+      uint32_t full_parity = 0u, empty_parity = 1u;
+      int s = (int)buf;
+      bool ok = true;
+#pragma unroll 1
+      for (int turn = (int)buf; turn < turns && ok; turn += 2) {
+        ok = mbar_wait(smem_u32(&sh.full[s]), full_parity, abort_flag);
+        const uint64_t a_desc = a_first + (uint64_t)(s * (int)(L8_STAGE >> 4)), b_desc = b_first + (uint64_t)(s * (int)(L8_STAGE >> 4));
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          ok = ok && mbar_wait(smem_u32(&sh.acc_empty[h][buf]), empty_parity, abort_flag);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t to = tmem_base + (uint32_t)(h * 2 + (int)buf) * 128u;
+#pragma unroll
+          for (int k = 0; k < L8_BK / 32; ++k) {      // 32 bytes further along the swizzled row: +2 in the 16-byte address field
+            // (a pair's half: 64 weight rows of each block)
+            if (PAIR) umma_e4m3_pair(to, a_desc + 2 * k, b_desc + (uint64_t)(h * (64 * L8_BK >> 4) + 2 * k), idesc, k != 0);
+            else umma_e4m3(to, a_desc + 2 * k, b_desc + 2 * k, idesc, k != 0);
+          }
+          if (PAIR) umma_commit_pair(smem_u32(&sh.acc_full[h][buf])); else umma_commit(smem_u32(&sh.acc_full[h][buf]));
+        }
+        if (!ok) break;
+        if (PAIR) umma_commit_pair(smem_u32(&sh.empty[s])); else umma_commit(smem_u32(&sh.empty[s]));
+        empty_parity ^= 1u;
+        if ((s += 2) >= a.stages) { s -= a.stages; full_parity ^= 1u; }
+      }
+    }
+  } else if (warp >= L8_FIRST) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L8_REGS_ADD));
+    constexpr int AHEAD = 4, WS = PAIR ? 2 : 1;
+    const int quad = warp & 3, group = (warp - L8_FIRST) / 4, h = PAIR ? group : 0;
+    // column i of the warp's sums: weight row n0 + col0 + i / 64 * 128 + i % 64
+    const int col0 = group * 64;
+    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(PAIR ? h * 256 : group * 64);
+    const uint32_t full0 = smem_u32(&sh.acc_full[h][0]), empty0 = PAIR ? mapa_u32(smem_u32(&sh.acc_empty[h][0]), 0u) : smem_u32(&sh.acc_empty[h][0]);
+    const uint32_t staged = smem_u32(tiles) + (uint32_t)a.stages * L8_STAGE + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
+    float x_ahead[AHEAD], w_ahead[WS][AHEAD];
+    const float *xs = a.xs, *ws = a.ws;
+    bool has_x = false, has_w[WS];
+    auto scales_of = [&](int tile) {      // of a tile's first blocks
+      if (tile >= tiles_all) return;
+      int n0, t0;
+      place(tile, n0, t0);
+      const int t = t0 + quad * 32 + lane;
+      has_x = t < a.T;
+      xs = a.xs + (size_t)k_first * a.T + (has_x ? t : 0);
+      ws = a.ws + (size_t)(n0 / L8_BK) * a.blocks + k_first;
+#pragma unroll
+      for (int i = 0; i < WS; ++i) has_w[i] = n0 + i * 128 < a.N;
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        x_ahead[d] = has_x && d < k_blocks ? xs[(size_t)d * a.T] : 0.f;
+#pragma unroll
+        for (int i = 0; i < WS; ++i) w_ahead[i][d] = has_w[i] && d < k_blocks ? ws[i * a.blocks + d] : 0.f;
+      }
+    };
+    scales_of(tile_first);
+    uint32_t turn = 0u;
+    bool ok = true;
+#pragma unroll 1
+    for (int tile = tile_first; tile < tiles_all; tile += tile_step) {
+      float2 acc[COLS / 2];
+#pragma unroll
+      for (int i = 0; i < COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+#pragma unroll 1
+      for (int k0 = 0; k0 < k_blocks && ok; k0 += AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+          const int kb = k0 + d;
+          if (kb >= k_blocks || !ok) break;
+          const uint32_t buf = turn & 1u, at = from + buf * 128u;
+          float f[WS];
+#pragma unroll
+          for (int i = 0; i < WS; ++i) f[i] = x_ahead[d] * w_ahead[i][d];
+          if (kb + AHEAD < k_blocks) {
+            if (has_x) x_ahead[d] = xs[(size_t)(kb + AHEAD) * a.T];
+#pragma unroll
+            for (int i = 0; i < WS; ++i)
+              if (has_w[i]) w_ahead[i][d] = ws[i * a.blocks + kb + AHEAD];
+          }
+          // tcgen05.ld is .sync.aligned: the lanes vote on the wait's answer
+          ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * buf, turn >> 1 & 1u, abort_flag) ? 1 : 0) != 0;
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          uint32_t v[2][16];
+          tmem_ld16(at, v[0]);
+#pragma unroll
+          for (int c = 0; c < COLS; c += 16) {
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (c + 16 < COLS) {
+              tmem_ld16(at + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
+            } else {
+              // all are read: the accumulator is free while the last of them are added
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
+                if (PAIR) l8_arrive_at(empty0 + 8u * buf); else l8_arrive(empty0 + 8u * buf);
+              }
+            }
+            const uint32_t(&u)[16] = v[(c / 16) & 1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) l8_fma2(acc[c / 2 + i], __uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), f[c / 64], f[c / 64]);
+          }
+          ++turn;
+        }
+      }
+      int n0, t0;
+      place(tile, n0, t0);
+      scales_of(tile + tile_step);
+      if (!ok) {
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) acc[i].x = acc[i].y = __int_as_float(L8_NONE);
+      }
+      const int row = quad * 32 + lane;
+      if (!PAIR && a.cut > 1) {
+        // all products are done, so the ring is free: this block's sums [128 tokens][128 + 4]
+        if (ok) {
+          float* part = reinterpret_cast<float*>(tiles) + row * (128 + 4) + col0;
+#pragma unroll
+          for (int i = 0; i < COLS / 4; ++i) *reinterpret_cast<float4*>(part + 4 * i) = make_float4(acc[2 * i].x, acc[2 * i].y, acc[2 * i + 1].x, acc[2 * i + 1].y);
+        }
+      } else if (boxes) {
+        // 32 rows of 128 bytes at a time, laid out as the copy's swizzle has them; two boxes take turns
+        constexpr int PER = 128 / (int)sizeof(O);
+#pragma unroll
+        for (int b = 0; b < COLS / PER; ++b) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the copy out of this box, two ago
+          __syncwarp();
+          const uint32_t box = staged + (uint32_t)(b & 1) * L8_BOX, to = box + (uint32_t)lane * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (sizeof(O) == 4) {
+                const int i = b * PER + c * 4 + e;
+                w[e] = __float_as_uint(i & 1 ? acc[i / 2].y : acc[i / 2].x);
+              } else {
+                const float2 p = acc[(b * PER + c * 8) / 2 + e];
+                const __nv_bfloat162 q = __floats2bfloat162_rn(p.x, p.y);
+                w[e] = *reinterpret_cast<const uint32_t*>(&q);
+              }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)((c ^ (lane & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            const int n = n0 + col0 + b * PER / 64 * 128 + b * PER % 64;
+            if (t0 + quad * 32 < a.T && n < a.N) l8_store_box(&tm_out, box, n, t0 + quad * 32);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
+      } else if (t0 + row < a.T) {
+        O* dst = out + (size_t)(t0 + row) * a.N;
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) {
+          const int n = n0 + col0 + i / 64 * 128 + i % 64;
+          if (n < a.N) dst[n] = qb_from_float<O>(i & 1 ? acc[i / 2].y : acc[i / 2].x);
+        }
+      }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (!PAIR && a.cut > 1) {
+    cluster_sync_all();
+    // a share of the rows; without the parts of a block that gave up they are no numbers
+    const bool missing = l8_missing(&sh.abort_flag, a.cut);
+    const uint32_t part = smem_u32(tiles);
+    int n0, t0;
+    place(tile_first, n0, t0);
+    const int share = 128 / a.cut, r_end = min((rank + 1) * share, a.T - t0);
+    for (int i = rank * share * 32 + (int)threadIdx.x; i < r_end * 32; i += L8_THREADS) {
+      const int row = i / 32, col = i % 32 * 4;
+      float4 sum = l8_sum_parts(part + 4u * (uint32_t)(row * (128 + 4) + col), a.cut);
+      if (missing) sum.x = sum.y = sum.z = sum.w = __int_as_float(L8_NONE);
+      l8_store4(out + (size_t)(t0 + row) * a.N, n0 + col, a.N, sum);
+    }
+  }
+  // no block leaves, or gives its accumulators back, while another's MMAs or sums may read what it has
+  if (PAIR || a.cut > 1) cluster_sync_all();
+  if (warp == 1) {
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
+  }
+  if (threadIdx.x == 0 && sh.abort_flag) qb_set_status(a.status, QB_STATUS_WAIT_TIMEOUT, tile_first, 11);
+}
+
+// [rows, cols] row-major, boxes of [box_rows] rows of 128 bytes
+int l8_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t size, uint32_t box_rows, CUtensorMapDataType type) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * size};
+  const cuuint32_t box[2] = {128 / size, box_rows};
+  return make_map(map, base, 2, dims, strides, box, type);
+}
+
+int l8_cluster_launch(const void* kern, void** args, unsigned grid, unsigned threads, unsigned width, size_t smem, cudaStream_t stream) {
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (err != cudaSuccess) return (int)err;
-  if (NT == 256) {
-    // the registers that the block's warps share out are those of the launch
-    cudaFuncAttributes attr;
-    err = cudaFuncGetAttributes(&attr, kern);
-    if (err != cudaSuccess) return (int)err;
-    if (attr.numRegs != L8_REGS_LAUNCH) return QB_ERR_UNSUPPORTED;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = l8_threads(NT);
+  cfg.blockDim = threads;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)a.cut;
+  attr[1].val.clusterDim.x = width;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  err = cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, a);
-  return (int)err;
+  return (int)cudaLaunchKernelExC(&cfg, kern, args);
+}
+
+template <int NT, typename O>
+int l8_few(CUtensorMap& tm_w, CUtensorMap& tm_x, LinearFp8& a, unsigned grid, size_t smem, cudaStream_t stream) {
+  void* args[] = {&tm_w, &tm_x, &a};
+  return l8_cluster_launch((const void*)linear_fp8_few_kernel<NT, O>, args, grid, L8_FEW_THREADS, (unsigned)a.cut, smem, stream);
+}
+template <bool PAIR, typename O>
+int l8_many(CUtensorMap& tm_w, CUtensorMap& tm_x, CUtensorMap& tm_out, LinearFp8& a, int boxes, unsigned grid, size_t smem, cudaStream_t stream) {
+  // the registers that the block's warps share out are those of the launch
+  const void* kern = (const void*)linear_fp8_kernel<PAIR, O>;
+  cudaFuncAttributes attr;
+  const cudaError_t err = cudaFuncGetAttributes(&attr, kern);
+  if (err != cudaSuccess) return (int)err;
+  if (attr.numRegs != L8_REGS_LAUNCH) return QB_ERR_UNSUPPORTED;
+  void* args[] = {&tm_w, &tm_x, &tm_out, &a, &boxes};
+  return l8_cluster_launch(kern, args, grid, L8_THREADS, PAIR ? 2u : (unsigned)a.cut, smem, stream);
 }
 
 }  // namespace
@@ -306,41 +663,68 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
                              int* status, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return QB_ERR_BAD_ARG;
+  if (out_dtype != QB_F32 && out_dtype != QB_BF16) return QB_ERR_BAD_ARG;
   int sms = 0;
   int rc = sm_count(sms);
   if (rc) return rc;
-  const int NT = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
   LinearFp8 a{xs, ws, out, T, K, N};
   a.blocks = (K + L8_BK - 1) / L8_BK;
-  a.t_tiles = (T + NT - 1) / NT;
-  const long long tiles = (long long)((N + L8_M - 1) / L8_M) * a.t_tiles;
+  a.status = status;
+  const CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  CUtensorMap tm_w, tm_x, tm_out;
+  if (T <= 64) {
+    const int NT = T <= 16 ? 16 : T <= 32 ? 32 : 64;
+    a.t_tiles = 1;
+    const long long tiles = (N + L8_M - 1) / L8_M;
+    a.cut = 1;
+    while (a.cut < 8 && tiles * a.cut < sms && a.blocks >= 4 * a.cut) a.cut *= 2;
+    a.per = (a.blocks + a.cut - 1) / a.cut;
+    const size_t stage = L8_A + (size_t)NT * L8_BK, need = a.cut > 1 ? (size_t)NT * L8_M * 4 : 0;
+    int stages = (int)(100 * 1024 / stage);
+    if (stages > L8_MAX_STAGES) stages = L8_MAX_STAGES;
+    if (stages > a.per) stages = a.per;
+    a.stages = stages;
+    const size_t ring = stage * stages, smem = (ring > need ? ring : need) + 1024;
+    rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, L8_M, bytes);
+    if (!rc) rc = l8_map(&tm_x, x, (uint64_t)T, (uint64_t)K, 1, (uint32_t)NT, bytes);
+    if (rc) return rc;
+    const unsigned grid = (unsigned)(tiles * a.cut);
+    QB_DISPATCH_DTYPE(out_dtype, O, {
+      if (NT == 16) rc = l8_few<16, O>(tm_w, tm_x, a, grid, smem, stream);
+      else if (NT == 32) rc = l8_few<32, O>(tm_w, tm_x, a, grid, smem, stream);
+      else rc = l8_few<64, O>(tm_w, tm_x, a, grid, smem, stream);
+    });
+    if (rc) return rc;
+    QB_LAUNCH_CHECK();
+    return 0;
+  }
+  // pairs of blocks where their tiles give every SM two turns or more, else tiles of 128 x 128, cut along k where they are few
+  const long long pair_tiles = (long long)((T + 255) / 256) * ((N + 255) / 256);
+  const bool pair = pair_tiles >= sms;
+  const int width = pair ? 256 : 128;
+  const size_t size = out_dtype == QB_F32 ? 4 : 2;
+  const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
+  a.t_tiles = (T + width - 1) / width;
+  const long long tiles = (long long)((N + width - 1) / width) * a.t_tiles;
   a.cut = 1;
-  while (a.cut < 8 && tiles * a.cut < sms && a.blocks >= 4 * a.cut) a.cut *= 2;
+  if (!pair)
+    while (a.cut < 8 && tiles * a.cut * 2 <= sms && a.blocks >= 4 * a.cut) a.cut *= 2;
   a.per = (a.blocks + a.cut - 1) / a.cut;
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
-  a.status = status;
-  const size_t stage = L8_A + (size_t)NT * L8_BK, need = a.cut > 1 ? (size_t)NT * L8_M * 4 : 0;
-  // one block an SM where the accumulators fill half of the TMEM or more
-  size_t room = NT >= 128 ? 200 * 1024 : 100 * 1024;
-  int stages = (int)(room / stage);
-  if (stages > L8_MAX_STAGES) stages = L8_MAX_STAGES;
-  if (stages > a.per) stages = a.per;
-  if (stages < 1) stages = 1;
-  a.stages = stages;
-  const size_t ring = stage * stages;
-  const size_t smem = (ring > need ? ring : need) + 1024;
-  CUtensorMap tm_w, tm_x;
-  rc = map_e4m3(&tm_w, w, (uint64_t)N, (uint64_t)K, L8_M);
+  const size_t stage = 2 * L8_A, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;
+  a.stages = a.cut > 1 ? 6 : 4;
+  const size_t ring = stage * a.stages, need = a.cut > 1 ? (size_t)128 * (128 + 4) * 4 : 0;
+  const size_t smem = (ring > need ? ring : need) + staged + 1024;
+  rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, 128, bytes);
+  if (!rc) rc = l8_map(&tm_x, x, (uint64_t)T, (uint64_t)K, 1, 128, bytes);
+  if (!rc && boxes)
+    rc = l8_map(&tm_out, out, (uint64_t)T, (uint64_t)N, (uint32_t)size, 32, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
   if (rc) return rc;
-  rc = map_e4m3(&tm_x, x, (uint64_t)T, (uint64_t)K, (uint32_t)NT);
-  if (rc) return rc;
-  const unsigned grid = (unsigned)(tiles * a.cut);
+  if (!boxes) tm_out = tm_x;      // not used
+  const unsigned grid = pair ? (unsigned)(sms / 2 * 2) : (unsigned)(tiles * a.cut);
   QB_DISPATCH_DTYPE(out_dtype, O, {
-    if (NT == 16) rc = l8_launch<16, O>(tm_w, tm_x, a, grid, smem, stream);
-    else if (NT == 32) rc = l8_launch<32, O>(tm_w, tm_x, a, grid, smem, stream);
-    else if (NT == 64) rc = l8_launch<64, O>(tm_w, tm_x, a, grid, smem, stream);
-    else if (NT == 128) rc = l8_launch<128, O>(tm_w, tm_x, a, grid, smem, stream);
-    else rc = l8_launch<256, O>(tm_w, tm_x, a, grid, smem, stream);
+    if (pair) rc = l8_many<true, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
+    else rc = l8_many<false, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
   });
   if (rc) return rc;
   QB_LAUNCH_CHECK();

@@ -208,7 +208,7 @@ def _product_within(out, x, xs, w, ws):
 
 PRODUCTS = [(1, 16, 1), (1, 128, 128), (1, 4096, 300), (2, 2048, 4096), (16, 144, 129), (17, 2048, 640), (32, 5632, 384), (33, 1040, 200), (64, 256, 77),
             (65, 11008, 256), (100, 272, 300), (128, 128, 128), (129, 4096, 257), (256, 640, 130), (300, 1040, 384), (513, 2048, 1000),
-            (700, 5648, 2000), (1025, 512, 40), (2500, 384, 2304)]
+            (700, 5648, 2000), (1025, 512, 40), (2500, 384, 2304), (2500, 400, 4001), (2561, 1280, 4104), (20000, 256, 640)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
