@@ -43,7 +43,7 @@ UNITS = {
     "state_space": ["selective_scan.cu"],
     "token_input": ["token_input.cu"],
     "decay_state": ["decay_state.cu"],
-    "fp8": ["fp8_rows.cu", "linear_fp8.cu"],
+    "fp8": ["fp8_rows.cu", "linear_fp8.cu", "linear_fp8_few.cu"],
     "scores": ["token_logprobs.cu"],
 }
 

@@ -5,7 +5,7 @@
 // (one rounding a block); two accumulators take turns, so that the tensor cores work on the next block meanwhile.  That addition has as
 // many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the two forms:
 //
-//  * up to 64 tokens (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
+//  * up to 64 tokens (linear_fp8_few_kernel; up to 16 linear_fp8_few.cu, mostly): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
 //    height of the MMA and the weights are read once.  A TMEM lane is a weight row, a column a token; the columns' scales come from shared memory.
 //  * more (linear_fp8_kernel): the tokens are the rows, the weights the columns.  A lane has its token's scale in a register and one weight
 //    scale for all of its columns, so the addition is one packed multiply-add for two numbers and reads nothing.  (With the tokens as columns the
@@ -659,6 +659,11 @@ int l8_many(CUtensorMap& tm_w, CUtensorMap& tm_x, CUtensorMap& tm_out, LinearFp8
 
 }  // namespace
 
+// linear_fp8_few.cu
+bool qb_linear_fp8_tokens_takes(int T, int K, int N, int sms);
+int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int sms,
+                         cudaStream_t stream);
+
 extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N,
                              int* status, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
@@ -667,6 +672,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   int sms = 0;
   int rc = sm_count(sms);
   if (rc) return rc;
+  if (qb_linear_fp8_tokens_takes(T, K, N, sms)) return qb_linear_fp8_tokens(x, xs, w, ws, out, out_dtype, T, K, N, sms, stream);
   LinearFp8 a{xs, ws, out, T, K, N};
   a.blocks = (K + L8_BK - 1) / L8_BK;
   a.status = status;
@@ -708,7 +714,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   const long long tiles = (long long)((N + width - 1) / width) * a.t_tiles;
   a.cut = 1;
   if (!pair)
-    while (a.cut < 8 && tiles * a.cut * 2 <= sms && a.blocks >= 4 * a.cut) a.cut *= 2;
+    while (a.cut < 4 && tiles * a.cut * 2 <= sms && a.blocks >= 4 * a.cut) a.cut *= 2;
   a.per = (a.blocks + a.cut - 1) / a.cut;
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
   const size_t stage = 2 * L8_A, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;

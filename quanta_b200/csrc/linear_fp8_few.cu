@@ -1,0 +1,173 @@
+// The product of linear_fp8.cu for at most 16 tokens, of a small matrix 32: bound by the bytes of w, and by what a launch costs besides them.
+//
+// A block takes 16 rows of w, its warps blocks of 128 k (one scale each) in turn.  A lane loads the 32 numbers of a row's 128 that it
+// then multiplies (the order of k inside an mma is free as long as both operands have it), 32 bytes a load, so that weights go from memory to
+// registers without shared memory, a barrier or tensor memory.  The four mma.sync of a block of 128 sum its products (of 8 bits each) in
+// float32, the sum is scaled by token and weight block and added in float32; the warps' parts are added in the order of the warps, so a
+// row's bits are the same in every step of as many warps a block.
+//
+// Measured on a B200, one product after another in a graph, weights from memory, microseconds (bytes at 6.5 TB/s / this / tcgen05): one token,
+// 4,096 x 22,016 13.8 / 18.2 / 18.3, 2,048 x 2,048 0.6 / 2.1 / 5.5; 8 tokens, 2,048 x 11,264 3.5 / 7.2 / 8.7, 5,632 x 2,048 1.8 / 4.5 / 7.5; 16 tokens,
+// 5,632 x 2,048 1.8 / 5.4 / 7.5, 4,096 x 22,016 13.8 / 21.3 / 19.3; 32 tokens, 2,048 x 2,048 0.6 / 3.9 / 6.2, 2,048 x 11,264 3.5 / 13 / 10.5.  What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps
+// and a cluster's parts before and behind the bytes; what bounds this one in a large matrix is the issue of instructions (154 a warp for 2 KB:
+// e4m3 operands of mma.sync are converted to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took
+// the same time; four pieces ahead instead of two a longer one (fewer warps).
+#include "fp8.cuh"
+
+namespace {
+
+
+
+struct LinearFp8Few {
+  const uint8_t *x, *w;
+  const float *xs, *ws;
+  void* out;
+  int T, K, N, blocks;
+};
+struct alignas(16) L8Piece {
+  uint32_t u[8];
+};
+
+// 32 bytes of a row, of which `left` (a multiple of 16) exist; WIDE: on 32 bytes and all there.  Weights are read once: not kept in L1.
+template <bool WIDE, bool ONCE>
+__device__ __forceinline__ L8Piece l8f_load(const uint8_t* p, int left) {
+  L8Piece v = {};
+  if (WIDE) {
+    if (left > 0) {
+      if (ONCE)
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7]) : "l"(p));
+      else
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7]) : "l"(p));
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (left > 16 * h)
+        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.u[4 * h]), "=r"(v.u[4 * h + 1]), "=r"(v.u[4 * h + 2]), "=r"(v.u[4 * h + 3]) : "l"(p + 16 * h));
+  }
+  return v;
+}
+
+__device__ __forceinline__ void l8f_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: tiles of 8 tokens.  D, XD: pieces of w and of x (with the scales) a warp holds ahead.
+template <int NT, int D, int XD, int WARPS, int MINB, bool WIDE, typename O>
+__global__ void __launch_bounds__(WARPS * 32, MINB) linear_fp8_tokens_kernel(LinearFp8Few a) {
+  static_assert(D % XD == 0, "the ring of x divides the ring of w");
+  qb_follow();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* wr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) wr[h] = a.w + (size_t)min(n0 + h * 8 + g, a.N - 1) * a.K + t * 32;
+  const uint8_t* xr[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) xr[n] = a.x + (size_t)min(n * 8 + g, a.T - 1) * a.K + t * 32;
+  const float* ws = a.ws + (size_t)(n0 / FP8_BLOCK) * a.blocks;
+  L8Piece wb[D][2], xb[XD][NT];
+  float xsb[XD][NT][2], wsb[XD];
+  auto fetch_w = [&](int kb, L8Piece (&b)[2]) {
+    const int left = kb < a.blocks ? a.K - kb * FP8_BLOCK - t * 32 : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) b[h] = l8f_load<WIDE, true>(wr[h] + kb * FP8_BLOCK, left);
+  };
+  auto fetch_x = [&](int kb, int at) {
+    const int left = kb < a.blocks ? a.K - kb * FP8_BLOCK - t * 32 : 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      xb[at][n] = l8f_load<WIDE, false>(xr[n] + kb * FP8_BLOCK, left);
+      // the scales of the tokens whose sums this lane has
+#pragma unroll
+      for (int i = 0; i < 2; ++i) xsb[at][n][i] = kb < a.blocks ? a.xs[(size_t)kb * a.T + min(n * 8 + 2 * t + i, a.T - 1)] : 0.f;
+    }
+    wsb[at] = kb < a.blocks ? ws[kb] : 0.f;
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch_w(warp + d * WARPS, wb[d]);
+#pragma unroll
+  for (int d = 0; d < XD; ++d) fetch_x(warp + d * WARPS, d);
+  float acc[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  for (int k0 = warp; k0 < a.blocks; k0 += D * WARPS) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int kb = k0 + d * WARPS;
+      if (kb >= a.blocks) break;
+      float c[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          l8f_mma(c[n], wb[d][0].u[2 * s], wb[d][1].u[2 * s], wb[d][0].u[2 * s + 1], wb[d][1].u[2 * s + 1], xb[d % XD][n].u[2 * s], xb[d % XD][n].u[2 * s + 1]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(c[n][i], xsb[d % XD][n][i & 1] * wsb[d % XD], acc[n][i]);
+      fetch_w(kb + D * WARPS, wb[d]);
+      fetch_x(kb + XD * WARPS, d % XD);
+    }
+  }
+  // the warps' parts, added in the order of the warps
+  constexpr int PAD = 20, TOK = NT * 8;
+  __shared__ float part[WARPS][TOK][PAD];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[warp][n * 8 + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[n][i];
+  __syncthreads();
+  for (int v = threadIdx.x; v < TOK * 16; v += WARPS * 32) {
+    const int tok = v / 16, row = v % 16;
+    if (tok >= a.T || n0 + row >= a.N) continue;
+    float s = part[0][tok][row];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) s += part[w][tok][row];
+    reinterpret_cast<O*>(a.out)[(size_t)tok * a.N + n0 + row] = qb_from_float<O>(s);
+  }
+}
+
+template <int NT, int D, int XD, int WARPS, int MINB, typename O>
+void l8f_launch(const LinearFp8Few& a, cudaStream_t stream) {
+  const int grid = (a.N + 15) / 16;
+  if (a.K % 32 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 31) == 0) qb_launch(linear_fp8_tokens_kernel<NT, D, XD, WARPS, MINB, true, O>, grid, WARPS * 32, 0, stream, a);
+  else qb_launch(linear_fp8_tokens_kernel<NT, D, XD, WARPS, MINB, false, O>, grid, WARPS * 32, 0, stream, a);
+}
+
+}  // namespace
+
+// Whether products of T tokens and a [N, K] matrix are this kernel's: up to 8 tokens all, up to 16 those of at most 32 MB, up to 32 those of a block
+// an SM and 12 MB at most.
+bool qb_linear_fp8_tokens_takes(int T, int K, int N, int sms) {
+  const long long bytes = (long long)K * N;
+  return T <= 8 || (T <= 16 && bytes <= 32 << 20) || (T <= 32 && (N + 15) / 16 <= sms && bytes <= 12 << 20);
+}
+
+// K a multiple of 16, x and w on 16 bytes (linear_fp8.cu has looked).  Blocks of four warps where there are two for every SM or
+// more, else of eight, so that few blocks have as many bytes on their way.
+int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int sms,
+                         cudaStream_t stream) {
+  const LinearFp8Few a{(const uint8_t*)x, (const uint8_t*)w, xs, ws, out, T, K, N, (K + FP8_BLOCK - 1) / FP8_BLOCK};
+  const bool many = (N + 15) / 16 >= 2 * sms;
+  QB_DISPATCH_DTYPE(out_dtype, O, {
+    if (T <= 8 && many) l8f_launch<1, 2, 2, 4, 4, O>(a, stream);
+    else if (T <= 8) l8f_launch<1, 2, 2, 8, 2, O>(a, stream);
+    else if (T <= 16 && many) l8f_launch<2, 2, 2, 4, 4, O>(a, stream);
+    else if (T <= 16) l8f_launch<2, 2, 2, 8, 2, O>(a, stream);
+    else l8f_launch<4, 2, 2, 8, 1, O>(a, stream);
+  });
+  QB_LAUNCH_CHECK();
+  return 0;
+}
