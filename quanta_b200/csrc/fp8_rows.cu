@@ -7,8 +7,7 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------
 // Row r (token tok = rows[r] if rows != null, else r):
-//   z = sum_s delta[tok, s, :]  (float32, s ascending);  with a gain g:  z = g * (z * rsqrt(mean(z^2) + eps_d))
-//   x = h[tok, :] + z;  if store_h: h[tok, :] = x
+//   x = h[tok, :] + sum_s delta[tok, s, :]  (float32, s ascending), or, with a gain g, h[tok, :] + g * (z * rsqrt(mean(z^2) + eps_d)) of their sum z;  if store_h: h[tok, :] = x
 //   out[r, :], scales[:, r] = e4m3 of w * (x * rsqrt(mean(x^2) + eps))
 // A tok outside the T rows of h gives a row of NaN.
 // ---------------------------------------------------------------------------------------------
@@ -40,10 +39,25 @@ __device__ __forceinline__ void fp8_no_row(const NormFp8& a, int r) {
   }
 }
 
+// x += the slots' eight numbers from column i on, slots in order
+template <typename D>
+__device__ __forceinline__ void fp8_add_slots(const NormFp8& a, int tok, int i, float (&x)[8]) {
+  const D* d = (const D*)a.delta + (size_t)tok * a.S * a.H + i;
+#pragma unroll 2
+  for (int s = 0; s < a.S; ++s) {
+    float dv[8];
+    QbVec8<D>::load(d + (size_t)s * a.H, dv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += dv[e];
+  }
+}
+
 // Rows of whole 32-byte pieces of at most 8,192 numbers: a thread keeps its 8 in registers from the load to the store, 16 threads hold a block
 // of 128 and find its largest among themselves.
-template <typename D, bool GAIN>
-__global__ void __launch_bounds__(1024) norm_fp8_rows_kernel(NormFp8 a) {
+// MOST: threads at most.  Without a gain the registers are held down to 32, so that an SM has the bytes of four rows on their way (8,192 rows of 4,096,
+// two float32 slots: 97 us with 40, 88 with 32; with a gain, and 40 instead of 56, they spill: 45 -> 59 us at 2,048).
+template <typename D, bool GAIN, int MOST>
+__global__ void __launch_bounds__(MOST, GAIN && MOST == 1024 ? 1 : 2) norm_fp8_rows_kernel(NormFp8 a) {
   qb_follow();
   __shared__ float scratch[2][32];
   const int r = blockIdx.x, tok = a.rows != nullptr ? a.rows[r] : r, i = threadIdx.x * 8;
@@ -52,49 +66,43 @@ __global__ void __launch_bounds__(1024) norm_fp8_rows_kernel(NormFp8 a) {
     fp8_no_row(a, r);
     return;
   }
-  float x[8], z[8], w[8];
+  float x[8], w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = z[e] = w[e] = 0.f;
-  if (in) {
-    QbVec8<float>::load(a.h + (size_t)tok * a.H + i, x);
-    QbVec8<float>::load(a.w + i, w);
-    if (a.delta != nullptr) {
-      const D* d = (const D*)a.delta + (size_t)tok * a.S * a.H + i;
-#pragma unroll 8
-      for (int s = 0; s < a.S; ++s) {
-        float dv[8];
-        QbVec8<D>::load(d + (size_t)s * a.H, dv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] += dv[e];
-      }
-    }
-  }
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
   if (GAIN) {
-    float g[8];
+    float z[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = 0.f;
-    if (in) QbVec8<float>::load(a.g + i, g);
+    for (int e = 0; e < 8; ++e) z[e] = w[e] = 0.f;
+    if (in) {
+      QbVec8<float>::load(a.h + (size_t)tok * a.H + i, x);
+      QbVec8<float>::load(a.g + i, w);
+      fp8_add_slots<D>(a, tok, i, z);
+    }
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss += z[e] * z[e];
     const float inv = rsqrtf(fp8_row_sum(ss, scratch[0]) / (float)a.H + a.eps_d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = g[e] * (z[e] * inv);
+    for (int e = 0; e < 8; ++e) x[e] += w[e] * (z[e] * inv);
+  } else if (in) {
+    QbVec8<float>::load(a.h + (size_t)tok * a.H + i, x);
+    if (a.delta != nullptr) fp8_add_slots<D>(a, tok, i, x);
   }
   float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] += z[e];
-    ss += x[e] * x[e];
-  }
+  for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
   if (in && a.store_h && a.delta != nullptr) QbVec8<float>::store(a.h + (size_t)tok * a.H + i, x);
+  // the gains are every block's, so they are near; asked for before the sum
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = 0.f;
+  if (in) QbVec8<float>::load(a.w + i, w);
   const float inv = rsqrtf(fp8_row_sum(ss, scratch[1]) / (float)a.H + a.eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = w[e] * (x[e] * inv);
   const float top = fp8_block_largest(fp8_largest(x));
   if (!in) return;
-  *reinterpret_cast<uint2*>(a.out + (size_t)r * a.H + i) = fp8_eight(x, FP8_TOP / top);
-  if ((threadIdx.x & 15) == 0) a.scales[(size_t)(i / FP8_BLOCK) * a.n + r] = top / FP8_TOP;
+  *reinterpret_cast<uint2*>(a.out + (size_t)r * a.H + i) = fp8_eight(x, fp8_up(top));
+  if ((threadIdx.x & 15) == 0) a.scales[(size_t)(i / FP8_BLOCK) * a.n + r] = fp8_scale(top);
 }
 
 // Any other row: held in shared memory between the passes, a warp a block of 128.
@@ -147,13 +155,13 @@ __global__ void __launch_bounds__(512) norm_fp8_any_kernel(NormFp8 a) {
     }
     top = fp8_max(top, __shfl_xor_sync(0xffffffffu, top, 16));
     top = fp8_block_largest(top);
-    const float up = FP8_TOP / top;
+    const float up = fp8_up(top);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = b * FP8_BLOCK + e * 32 + lane;
       if (i < a.H) a.out[(size_t)r * a.H + i] = fp8_one(v[e] * up);
     }
-    if (lane == 0) a.scales[(size_t)b * a.n + r] = top / FP8_TOP;
+    if (lane == 0) a.scales[(size_t)b * a.n + r] = fp8_scale(top);
   }
 }
 
@@ -170,74 +178,137 @@ struct ActFp8 {
   float limit, alpha;
 };
 
+__device__ __forceinline__ float fp8_min(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The exponential and the reciprocal are the fast ones (some 2 ulp, and 2^-23 of the argument): what follows is rounded to four bits.
+__device__ __forceinline__ float2 fp8_sigmoid2(float2 g, float by) {      // 1 / (1 + e^(-g by / log2 e))
+  const float2 z = fp8_mul2(g, make_float2(-by, -by));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
+  e = fp8_add2(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+  return e;
+}
+// Two numbers at a time: the kernel is bound by the issue of instructions (an activation with biases and clamps) as much as by memory.
 template <int KIND>
-__device__ __forceinline__ float act_one(float g, float u, float limit, float alpha) {
+__device__ __forceinline__ float2 act_two(float2 g, float2 u, float limit, float alpha) {
+  constexpr float LOG2E = 1.4426950408889634f;
   if (KIND == ACT_CLAMPED) {
-    g = g > limit ? limit : g;                                        // (a NaN stays one)
-    u = u > limit ? limit : u < -limit ? -limit : u;
-    return g / (1.f + expf(-alpha * g)) * (u + 1.f);
+    g = make_float2(fp8_min(g.x, limit), fp8_min(g.y, limit));      // (a NaN stays one)
+    u = make_float2(fp8_max(fp8_min(u.x, limit), -limit), fp8_max(fp8_min(u.y, limit), -limit));
+    const float2 t = fp8_mul2(g, fp8_sigmoid2(g, alpha * LOG2E));
+    return fp8_fma2(u, t, t);
   }
-  if (KIND == ACT_GELU) return qb_gelu_tanh(g) * u;
-  if (KIND == ACT_SILU) return g / (1.f + expf(-g)) * u;
+  if (KIND == ACT_GELU) {      // as qb_gelu_tanh
+    const float2 t = fp8_fma2(fp8_mul2(g, g), fp8_mul2(g, make_float2(0.044715f, 0.044715f)), g);
+    return fp8_mul2(fp8_mul2(g, fp8_sigmoid2(t, 1.5957691216057308f * LOG2E)), u);
+  }
+  if (KIND == ACT_SILU) return fp8_mul2(fp8_mul2(g, fp8_sigmoid2(g, LOG2E)), u);
   return g;
 }
 
-constexpr int ACT_THREADS = 256, ACT_COLS = ACT_THREADS * 8;
-// VEC: whole 16-byte pieces.  Sixteen threads hold a block of 128 columns, eight numbers each; a thread takes the same columns of several rows.
-template <typename T, int KIND, bool VEC>
-__global__ void __launch_bounds__(ACT_THREADS) act_fp8_kernel(ActFp8 a) {
+// Sixteen threads hold a block of 128 columns, eight numbers each, and take the same columns of neighbouring rows: the biases stay in registers,
+// the numbers of several rows (128 bytes a thread) are on their way together, and the rows' scales of a block are neighbours.  VEC: whole 16-byte
+// pieces; else neighbouring threads take neighbouring numbers of the block.
+constexpr int ACT_THREADS = 256, ACT_COLS = ACT_THREADS * 8, ACT_ROWS = 8;
+template <typename T, int KIND, bool BIAS, bool VEC>
+__global__ void __launch_bounds__(ACT_THREADS) act_fp8_kernel(ActFp8 a, int rows_each) {
   qb_follow();
-  const int c = blockIdx.x * ACT_COLS + threadIdx.x * 8;
-  const int width = KIND == ACT_NONE ? a.I : 2 * a.I;
-  const T* x = (const T*)a.x;
-  for (int r = blockIdx.y; r < a.n; r += gridDim.y) {
-    float g[8], u[8];
-    const T* row = x + (size_t)r * width;
-    if (VEC) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = u[e] = 0.f;
-      if (c < a.I) {
-        QbVec8<T>::load(row + c, g);
-        if (KIND != ACT_NONE) QbVec8<T>::load(row + a.I + c, u);
-        if (KIND != ACT_NONE && a.bias != nullptr) {
-          float bg[8], bu[8];
-          QbVec8<float>::load(a.bias + c, bg);
-          QbVec8<float>::load(a.bias + a.I + c, bu);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) { g[e] += bg[e]; u[e] += bu[e]; }
-        }
-      }
+  constexpr int AHEAD = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2, PIECES = VEC ? (int)sizeof(T) / 2 : 1;
+  const int c = blockIdx.x * ACT_COLS + threadIdx.x * 8, c0 = c / FP8_BLOCK * FP8_BLOCK + (threadIdx.x & 15);
+  const bool in = c < a.I;
+  const size_t width = KIND == ACT_NONE ? a.I : 2 * (size_t)a.I;
+  auto column = [&](int e) { return VEC ? c + e : c0 + e * 16; };
+  float bg[8], bu[8];
+  if (BIAS) {
+    if (VEC && in) {
+      QbVec8<float>::load(a.bias + c, bg);
+      QbVec8<float>::load(a.bias + a.I + c, bu);
     } else {
-      // neighbouring threads take neighbouring numbers of the block
-      const int c0 = c / FP8_BLOCK * FP8_BLOCK + (threadIdx.x & 15);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int i = c0 + e * 16;
-        g[e] = i < a.I ? qb_to_float<T>(row[i]) : 0.f;
-        u[e] = KIND != ACT_NONE && i < a.I ? qb_to_float<T>(row[a.I + i]) : 0.f;
-        if (KIND != ACT_NONE && a.bias != nullptr && i < a.I) { g[e] += a.bias[i]; u[e] += a.bias[a.I + i]; }
+        const bool has = !VEC && column(e) < a.I;
+        bg[e] = has ? a.bias[column(e)] : 0.f;
+        bu[e] = has ? a.bias[a.I + column(e)] : 0.f;
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = act_one<KIND>(g[e], u[e], a.limit, a.alpha);
-    const float top = fp8_block_largest(fp8_largest(g)), up = FP8_TOP / top;
+  }
+  const int r_end = min(a.n, ((int)blockIdx.y + 1) * rows_each);
+#pragma unroll 1
+  for (int r0 = blockIdx.y * rows_each; r0 < r_end; r0 += AHEAD) {
+    uint4 raw[AHEAD][2][PIECES];
     if (VEC) {
-      if (c < a.I) *reinterpret_cast<uint2*>(a.out + (size_t)r * a.I + c) = fp8_eight(g, up);
-    } else {
-      const int c0 = c / FP8_BLOCK * FP8_BLOCK + (threadIdx.x & 15);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e * 16 < a.I) a.out[(size_t)r * a.I + c0 + e * 16] = fp8_one(g[e] * up);
+      for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+          raw[d][0][p] = raw[d][1][p] = make_uint4(0u, 0u, 0u, 0u);
+          if (!in || r0 + d >= r_end) continue;
+          const uint4* row = reinterpret_cast<const uint4*>((const T*)a.x + (size_t)(r0 + d) * width + c);
+          raw[d][0][p] = row[p];
+          if (KIND != ACT_NONE) raw[d][1][p] = row[(size_t)a.I * sizeof(T) / 16 + p];
+        }
     }
-    if ((threadIdx.x & 15) == 0 && c < a.I) a.scales[(size_t)(c / FP8_BLOCK) * a.n + r] = top / FP8_TOP;
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      const int r = r0 + d;
+      if (r >= r_end) break;
+      float g[8], u[8];
+      if (VEC) {
+        QbVec8<T>::load(reinterpret_cast<const T*>(raw[d][0]), g);
+        QbVec8<T>::load(reinterpret_cast<const T*>(raw[d][1]), u);
+      } else {
+        const T* row = (const T*)a.x + (size_t)r * width;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = column(e);
+          g[e] = i < a.I ? qb_to_float<T>(row[i]) : 0.f;
+          u[e] = KIND != ACT_NONE && i < a.I ? qb_to_float<T>(row[a.I + i]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        float2 g2 = make_float2(g[e], g[e + 1]), u2 = make_float2(u[e], u[e + 1]);
+        if (BIAS) {
+          g2 = fp8_add2(g2, make_float2(bg[e], bg[e + 1]));
+          u2 = fp8_add2(u2, make_float2(bu[e], bu[e + 1]));
+        }
+        g2 = act_two<KIND>(g2, u2, a.limit, a.alpha);
+        g[e] = g2.x;
+        g[e + 1] = g2.y;
+      }
+      const float top = fp8_block_largest(fp8_largest(g)), up = fp8_up(top);
+      if (VEC) {
+        if (in) *reinterpret_cast<uint2*>(a.out + (size_t)r * a.I + c) = fp8_eight(g, up);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (column(e) < a.I) a.out[(size_t)r * a.I + column(e)] = fp8_one(g[e] * up);
+      }
+      if ((threadIdx.x & 15) == 0 && in) a.scales[(size_t)(c / FP8_BLOCK) * a.n + r] = fp8_scale(top);
+    }
   }
 }
 
+template <typename T, int KIND, bool BIAS>
+void act_fp8_launch(const ActFp8& a, bool vec, cudaStream_t stream) {
+  // few rows: one a block, so that more SMs take part; a grid has 65,535 rows of blocks at most
+  const int across = (a.I + ACT_COLS - 1) / ACT_COLS;
+  int rows = (long long)a.n * across >= 148 * 8 * ACT_ROWS ? ACT_ROWS : 1;
+  while ((a.n + rows - 1) / rows > 65535) rows *= 2;
+  const dim3 grid(across, (a.n + rows - 1) / rows);
+  if (vec) qb_launch(act_fp8_kernel<T, KIND, BIAS, true>, grid, ACT_THREADS, 0, stream, a, rows);
+  else qb_launch(act_fp8_kernel<T, KIND, BIAS, false>, grid, ACT_THREADS, 0, stream, a, rows);
+}
 template <typename T, int KIND>
 void act_fp8_launch(const ActFp8& a, bool vec, cudaStream_t stream) {
-  const dim3 grid((a.I + ACT_COLS - 1) / ACT_COLS, a.n < 32768 ? a.n : 32768);
-  if (vec) qb_launch(act_fp8_kernel<T, KIND, true>, grid, ACT_THREADS, 0, stream, a);
-  else qb_launch(act_fp8_kernel<T, KIND, false>, grid, ACT_THREADS, 0, stream, a);
+  if (KIND != ACT_NONE && a.bias != nullptr) act_fp8_launch<T, KIND, KIND != ACT_NONE>(a, vec, stream);
+  else act_fp8_launch<T, KIND, false>(a, vec, stream);
 }
 
 }  // namespace
@@ -250,8 +321,9 @@ extern "C" int qb_add_rmsnorm_fp8(float* h, const void* delta, int delta_dtype, 
   if (H % 8 == 0 && H <= 8192 && (((uintptr_t)h | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)g) & 15) == 0 && ((uintptr_t)out & 7) == 0) {
     const int threads = (H / 8 + 31) / 32 * 32;
     QB_DISPATCH_DTYPE(delta_dtype, D, {
-      if (g != nullptr) qb_launch(norm_fp8_rows_kernel<D, true>, n_rows, threads, 0, stream, a);
-      else qb_launch(norm_fp8_rows_kernel<D, false>, n_rows, threads, 0, stream, a);
+      if (g != nullptr && threads <= 512) qb_launch(norm_fp8_rows_kernel<D, true, 512>, n_rows, threads, 0, stream, a);
+      else if (g != nullptr) qb_launch(norm_fp8_rows_kernel<D, true, 1024>, n_rows, threads, 0, stream, a);
+      else qb_launch(norm_fp8_rows_kernel<D, false, 1024>, n_rows, threads, 0, stream, a);
     });
     QB_LAUNCH_CHECK();
     return 0;
