@@ -17,6 +17,7 @@ import torch
 from ..sampling.sampler import Sampler
 from .model import Model, load_model
 from .scheduler import PlannedEntry, Request, SamplingParams, Scheduler
+from .score import TextScores, score_texts
 from .step import Engine, StepEntry
 
 
@@ -34,18 +35,22 @@ class LLM:
 
     ``num_pages`` pages of ``page_size`` tokens are shared by all live requests; ``max_requests`` is the
     number of state slots; a step carries at most ``max_step_tokens`` tokens, a prompt portion at most
-    ``prefill_chunk``.
+    ``prefill_chunk``.  ``dense_weights`` ``"fp8"`` (for a model folder): the gated dense feed-forwards' matrices in 8 bits
+    (``Model``).
     """
 
     def __init__(self, model, *, dtype="bfloat16", device="cuda:0", page_size: int = 16,
                  num_pages: int | None = None, max_requests: int = 64, max_step_tokens: int = 4096,
-                 prefill_chunk: int = 4096, max_position: int | None = None):
+                 prefill_chunk: int = 4096, max_position: int | None = None,
+                 dense_weights: str | None = None):
         if isinstance(model, (str, Path)):
-            model, cfg = load_model(model, dtype=dtype, device=device)
+            model, cfg = load_model(model, dtype=dtype, device=device, dense_weights=dense_weights)
             self.config = cfg
             if max_position is None:
                 max_position = getattr(cfg, "max_position_embeddings", None)
         elif isinstance(model, Model):
+            if dense_weights is not None:
+                raise ValueError("dense_weights is for a model folder; a Model was made with its own")
             self.config = None
         else:
             raise TypeError("model must be a model folder or a loaded Model")
@@ -77,6 +82,15 @@ class LLM:
         self.run(reqs)
         outs = [r.generated for r in reqs]
         return outs[0] if single else outs
+
+    def score(self, texts, *, top: int = 0) -> list:
+        """How probable ``texts`` (one list of token ids, or a list of such lists) are: a ``TextScores`` for each (one, if ``texts`` is one),
+        with every token's log probability after those before it, the entropies there, and the ``top`` most probable tokens."""
+        single = bool(texts) and not isinstance(texts[0], (list, tuple))
+        many = [list(texts)] if single else [list(t) for t in texts]
+        out: list[TextScores] = score_texts(self.engine, many, top=top, max_position=self.sched_opts["max_position"],
+                                            max_tokens=min(self.sched_opts["max_step_tokens"], self.sched_opts["prefill_chunk"]))
+        return out[0] if single else out
 
     def _decode_ahead(self, sched: Scheduler, plan: list) -> list | None:
         """The requests of the decode step that follows ``plan`` if that step can be launched before
@@ -181,7 +195,7 @@ def generate(model, prompt_ids, *, max_new_tokens: int, temperature: float = 0.0
     """Generate up to ``max_new_tokens`` ids after ``prompt_ids``; stops early on ``eos_id`` (an int
     or a collection; default: the model's own eos ids).  ``model`` is a model folder or an ``LLM``;
     ``prompt_ids`` one prompt or a list of prompts.  ``engine_options`` (dtype, page_size, num_pages,
-    max_requests, max_step_tokens, prefill_chunk) apply when ``model`` is a folder."""
+    max_requests, max_step_tokens, prefill_chunk, dense_weights) apply when ``model`` is a folder."""
     llm = model if isinstance(model, LLM) else LLM(model, **engine_options)
     first = prompt_ids[0] if len(prompt_ids) else None
     if first is None or (isinstance(first, (list, tuple)) and any(len(p) == 0 for p in prompt_ids)):

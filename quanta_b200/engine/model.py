@@ -63,14 +63,21 @@ def _walk(part: Part):
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, dtype=torch.bfloat16, device="cuda:0"):
+    def __init__(self, spec: ModelSpec, dtype=torch.bfloat16, device="cuda:0", dense_weights: str | None = None):
+        """``dense_weights`` ``"fp8"``: the matrices of the parts that can hold theirs in 8 bits (the gated dense feed-forwards) are brought to e4m3
+        with a scale for every 128 x 128 numbers as they are loaded; a model without such a part is refused."""
+        if dense_weights not in (None, "fp8"):
+            raise ValueError(f"dense_weights {dense_weights!r}: choose \"fp8\", or None for the model's dtype")
         self.spec = spec
+        self.dense_weights = dense_weights
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
         self.embedding = make("embedding", spec.embedding)
         self.blocks = [make("block", choice) for choice in spec.layers]
         self.head = make("head", spec.head)
         self.schedule = list(spec.schedule)
+        if dense_weights is not None and not any(hasattr(p, "hold_in_fp8") for p in self.parts()):
+            raise ValueError(f"dense_weights {dense_weights!r}: {spec.name} has no gated dense feed-forward, whose weights could be held so")
         self.loaded = False
         # a list to have ``forward`` append the residual stream after every schedule entry (float32 [T, hidden]
         # copies; costs a kernel and memory per entry, and keeps steps out of captured graphs' fast path)
@@ -113,6 +120,8 @@ class Model:
 
         for p in self.parts():
             p.load(fetch_shared)
+            if self.dense_weights == "fp8" and hasattr(p, "hold_in_fp8"):
+                p.hold_in_fp8()
         self.loaded = True
         return self
 
@@ -151,12 +160,12 @@ class Model:
 
 
 # ------------------------------------------------------------------------------------------------
-def load_model(model_dir, dtype="bfloat16", device="cuda:0") -> tuple[Model, object]:
-    """Model folder (config.json + safetensors) -> (loaded model, its configuration)."""
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", dense_weights: str | None = None) -> tuple[Model, object]:
+    """Model folder (config.json + safetensors) -> (loaded model, its configuration).  ``dense_weights``: as for ``Model``."""
     from .. import models  # noqa: F401  (registers the architectures)
     matmul.configure()
     arch, cfg = load_config(model_dir)
-    model = Model(arch.build_spec(cfg), dtype=dtype, device=device)
+    model = Model(arch.build_spec(cfg), dtype=dtype, device=device, dense_weights=dense_weights)
     src = FolderSource(model_dir)
     try:
         model.load(src)
@@ -165,13 +174,13 @@ def load_model(model_dir, dtype="bfloat16", device="cuda:0") -> tuple[Model, obj
     return model, cfg
 
 
-def random_model(cfg, seed: int, dtype="bfloat16", device="cuda:0", arch=None) -> Model:
+def random_model(cfg, seed: int, dtype="bfloat16", device="cuda:0", arch=None, dense_weights: str | None = None) -> Model:
     """Seeded random weights generated on the device, no files (for sizes too large to write)."""
     from .. import models  # noqa: F401
     from ..config.registry import resolve
     matmul.configure()
     arch = arch or resolve(cfg.to_dict())
-    model = Model(arch.build_spec(cfg), dtype=dtype, device=device)
+    model = Model(arch.build_spec(cfg), dtype=dtype, device=device, dense_weights=dense_weights)
     model.load(RandomSource(model.tensor_specs(), seed, matrix_dtype=torch.bfloat16))
     return model
 

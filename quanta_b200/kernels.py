@@ -1260,11 +1260,40 @@ FP8_BLOCK = 128                 # columns of a row, and rows and columns of a we
 E4M3 = torch.float8_e4m3fn
 
 
-def _here(what: str, **tensors) -> None:
-    """All of them on the current device (the kernel is launched on its stream)."""
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
-            raise ValueError(f"{what}: {name} is on {t.device}, which is not the current CUDA device")
+_VOID, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+
+
+_ENTRIES: dict = {}
+
+
+def _entry(name: str, types: str):
+    """An entry point that takes plain numbers.  Their types (p pointer, i int, l long long, f float) are told to ctypes once: a call of a few
+    microseconds is mostly its arguments."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = [{"p": _VOID, "i": _INT, "l": _LONG, "f": _FLOAT}[t] for t in types]
+        _ENTRIES[name] = fn
+    return fn
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _addresses(what: str, names: tuple, tensors: tuple, strided: int = -1) -> tuple[int, list]:
+    """The current device, and the tensors' addresses (None stays None): all of them there, and contiguous but for number ``strided``, whose caller
+    has looked at its strides.  The first is no None."""
+    device = tensors[0].get_device()
+    if device < 0 or device != _current_device():
+        raise ValueError(f"{what}: {names[0]} is on {tensors[0].device}, which is not the current CUDA device")
+    for i, t in enumerate(tensors):
+        if t is not None and (t.get_device() != device or not (t.is_contiguous() or i == strided)):
+            raise ValueError(f"{what}: {names[i]} must be contiguous and on {tensors[0].device}, it is on {t.device}")
+    return device, [None if t is None else t.data_ptr() for t in tensors]
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, cols: int, name: str) -> None:
@@ -1303,10 +1332,11 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: torch.Tensor | None, weight: torch.T
     if weight.numel() != H:
         raise ValueError("add_rmsnorm_fp8: weight shape mismatch")
     _fp8_rows("add_rmsnorm_fp8", out, scales, n, H, "out")
-    _here("add_rmsnorm_fp8", h=h, delta=delta, weight=weight, delta_gain=delta_gain, out=out, scales=scales, rows=rows)
-    _check(lib().qb_add_rmsnorm_fp8(_p(h), _p(delta), _code(delta) if delta is not None else F32, S, _p(weight), _p(delta_gain), _p(out),
-                                    _p(scales), _p(rows), n, T, H, ctypes.c_float(eps), ctypes.c_float(delta_eps), int(store_h), _stream()),
-           "add_rmsnorm_fp8")
+    device, (p_h, p_delta, p_w, p_gain, p_out, p_scales, p_rows) = _addresses(
+        "add_rmsnorm_fp8", ("h", "delta", "weight", "delta_gain", "out", "scales", "rows"), (h, delta, weight, delta_gain, out, scales, rows))
+    fn = _entry("qb_add_rmsnorm_fp8", "ppiipppppiiiffip")
+    _check(fn(p_h, p_delta, _code(delta) if delta is not None else F32, S, p_w, p_gain, p_out, p_scales, p_rows, n, T, H, eps, delta_eps,
+              int(store_h), _stream_of(device)), "add_rmsnorm_fp8")
 
 
 def glu_act_fp8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, *, bias: torch.Tensor | None = None, kind: int = GLU_SILU,
@@ -1325,9 +1355,13 @@ def glu_act_fp8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, 
     if kind == GLU_CLAMPED and not limit > 0:
         raise ValueError("glu_act_fp8: the clamped form needs a positive limit")
     _fp8_rows("glu_act_fp8", out, scales, n, two_i // 2, "out")
-    _here("glu_act_fp8", gate_up=gate_up, bias=bias, out=out, scales=scales)
-    _check(lib().qb_act_fp8(_p(gate_up), _code(gate_up), _p(bias), _p(out), _p(scales), n, two_i // 2, int(kind), ctypes.c_float(limit),
-                            ctypes.c_float(alpha), _stream()), "glu_act_fp8")
+    _act_fp8("glu_act_fp8", gate_up, bias, out, scales, two_i // 2, kind, limit, alpha)
+
+
+def _act_fp8(what: str, x, bias, out, scales, cols: int, kind: int, limit: float, alpha: float) -> None:
+    device, (p_x, p_bias, p_out, p_scales) = _addresses(what, ("the input", "bias", "out", "scales"), (x, bias, out, scales))
+    fn = _entry("qb_act_fp8", "pipppiiiffp")
+    _check(fn(p_x, _code(x), p_bias, p_out, p_scales, x.shape[0], cols, int(kind), limit, alpha, _stream_of(device)), what)
 
 
 def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1336,9 +1370,7 @@ def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> Non
         raise ValueError("rows_to_fp8: x must be [n, K]")
     n, K = x.shape
     _fp8_rows("rows_to_fp8", out, scales, n, K, "out")
-    _here("rows_to_fp8", x=x, out=out, scales=scales)
-    _check(lib().qb_act_fp8(_p(x), _code(x), _p(None), _p(out), _p(scales), n, K, 3, ctypes.c_float(0.0), ctypes.c_float(1.0), _stream()),
-           "rows_to_fp8")
+    _act_fp8("rows_to_fp8", x, None, out, scales, K, 3, 0.0, 1.0)
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
@@ -1361,8 +1393,10 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError(f"linear_fp8: K must be a positive multiple of 16, got {K}")
     if status is not None:
         _want(status, torch.int32, "status")
-    _here("linear_fp8", x=x, x_scales=x_scales, w=w, w_scales=w_scales, out=out, status=status)
-    _check(lib().qb_linear_fp8(_p(x), _p(x_scales), _p(w), _p(w_scales), _p(out), _code(out), T, K, N, _p(status), _stream()), "linear_fp8")
+    device, (p_x, p_xs, p_w, p_ws, p_out, p_status) = _addresses(
+        "linear_fp8", ("x", "x_scales", "w", "w_scales", "out", "status"), (x, x_scales, w, w_scales, out, status))
+    fn = _entry("qb_linear_fp8", "pppppiiiipp")
+    _check(fn(p_x, p_xs, p_w, p_ws, p_out, _code(out), T, K, N, p_status, _stream_of(device)), "linear_fp8")
 
 
 TOKEN_LOGPROBS_MAX_TOP = 64
@@ -1400,10 +1434,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
             raise ValueError(f"token_logprobs: {top} tokens a row of {V}; at most {TOKEN_LOGPROBS_MAX_TOP} are taken, and no more than there are")
     if status is not None:
         _want(status, torch.int32, "status")
-    _here("token_logprobs", logits=logits, tokens=tokens, logprob=logprob, entropy=entropy, ids=ids, best=best, status=status)
-    _check(lib().qb_token_logprobs(ctypes.c_void_p(logits.data_ptr()), _code(logits), ctypes.c_longlong(logits.stride(0)), _p(tokens), _p(logprob),
-                                   _p(entropy), _p(ids if top else None), _p(best if top else None), n, V, top, _p(status), _stream()),
-           "token_logprobs")
+    device, (p_x, p_t, p_lp, p_en, p_ids, p_best, p_status) = _addresses(
+        "token_logprobs", ("logits", "tokens", "logprob", "entropy", "ids", "best", "status"),
+        (logits, tokens, logprob, entropy, ids if top else None, best if top else None, status), strided=0)
+    fn = _entry("qb_token_logprobs", "pilpppppiiipp")
+    _check(fn(p_x, _code(logits), logits.stride(0), p_t, p_lp, p_en, p_ids, p_best, n, V, top, p_status, _stream_of(device)), "token_logprobs")
 
 
 def split2_bf16(x) -> torch.Tensor:

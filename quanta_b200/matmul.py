@@ -1,5 +1,6 @@
 """Dense projections (``nn.Linear`` in the reference, src/quanta/minimax/attention.py:166-169): products of a few rows by the framework's
-own kernels (``csrc/linear_few.cu`` in bfloat16, ``csrc/linear_rows.cu`` in float32), the others by the library's (cuBLAS via torch).
+own kernels (``csrc/linear_few.cu`` in bfloat16, ``csrc/linear_rows.cu`` in float32), the others by the library's (cuBLAS via torch); products of
+8-bit operands with scales by its own ones for any number of rows (``csrc/linear_fp8.cu``).
 
 float32 products run as true float32: TF32 and reduced-precision accumulation are switched off
 process-wide when the first engine is built.
@@ -12,6 +13,7 @@ import torch.autograd.forward_ad as forward_ad
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import kernels
+from .fp8 import Fp8Rows, Fp8Weight, quantize_rows
 
 _configured = False
 
@@ -100,6 +102,16 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
     if out_dtype is not None and out_dtype != x.dtype:
         return torch.mm(x, w.t(), out_dtype=out_dtype)
     return torch.mm(x, w.t())
+
+
+def linear_fp8(x: Fp8Rows | torch.Tensor, w: Fp8Weight, out_dtype: torch.dtype, ctx=None) -> torch.Tensor:
+    """``x [T, in] @ w [out, in].T`` of 8-bit operands (``x``, if it is a tensor, is brought to 8 bits first); sums are float32, rounded once
+    to ``out_dtype``.  ``ctx``: the step's context, whose status words record a wait in the kernel that ran out."""
+    if not isinstance(x, Fp8Rows):
+        x = quantize_rows(x)
+    out = torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype, device=x.q.device)
+    kernels.linear_fp8(x.q, x.scales, w.q, w.scales, out, getattr(ctx, "status", None))
+    return out
 
 
 def linear_silu(x: torch.Tensor, w: torch.Tensor, ctx=None) -> torch.Tensor | None:

@@ -34,7 +34,7 @@ class PreNormBlock(Block):
         x = empty_rows(h.shape[0], self.hidden, dtype=ctx.dtype, device=h.device)
         self.mixer_norm.forward(h, pending, x)
         a = self.mixer.forward(x, ctx, cache, state)
-        x2 = empty_rows(h.shape[0], self.hidden, dtype=ctx.dtype, device=h.device)
+        x2 = _norms.rows_for(self.feed_forward, self.feed_forward_norm, h, self.hidden, ctx.dtype)
         self.feed_forward_norm.forward(h, a, x2)
         return self.feed_forward.forward(x2, ctx)
 
@@ -107,7 +107,7 @@ class SandwichNormBlock(Block):
         d = NormedPending(self.mixer.forward(x, ctx, cache, state), self.mixer_post_norm)
         if self.feed_forward is None:
             return d
-        x2 = empty_rows(T, self.hidden, dtype=ctx.dtype, device=h.device)
+        x2 = _norms.rows_for(self.feed_forward, self.feed_forward_norm, h, self.hidden, ctx.dtype)
         self.feed_forward_norm.forward(h, d, x2)
         return NormedPending(self.feed_forward.forward(x2, ctx), self.feed_forward_post_norm)
 

@@ -2,6 +2,9 @@
 the three projections), or in the clamped form ``g = min(gate x, limit)``, ``u = clamp(up x, -limit, limit)``,
 ``down(g * sigmoid(alpha g) * (u + 1))``, or with the tanh form of gelu for silu; and ungated, ``down(act(up x))`` with ``act`` the square of relu.
 
+A gated feed-forward's matrices may be held in 8 bits (``hold_in_fp8``): it then reads 8-bit rows, which the norm before it writes where the block
+hands them on (``reads_fp8``), or brings its input to 8 bits itself.
+
 The gate and up matrices are held as one, so a step is two library products and one activation kernel.
 The result is float32 (the accumulator of the down product), for blocks that norm it before the sum.
 """
@@ -11,7 +14,8 @@ from __future__ import annotations
 import torch
 
 from .. import kernels
-from ..matmul import empty_rows, linear, linear_silu
+from ..fp8 import Fp8Weight, empty_rows as empty_fp8_rows, quantize_weight
+from ..matmul import empty_rows, linear, linear_fp8, linear_silu
 from .base import Addends, FeedForward, TensorSpec, register
 
 
@@ -53,7 +57,27 @@ class GatedDense(FeedForward):
             self.b_gate_up = torch.cat([fetch(self.names["gate_b"]), fetch(self.names["up_b"])]).contiguous()
             self.b_down = fetch(self.names["down_b"]).contiguous()
 
+    def hold_in_fp8(self) -> None:
+        """Bring the loaded matrices to 8 bits (e4m3, a scale for every 128 x 128 numbers); the biases stay float32."""
+        if self.hidden % 16 or self.inner % 16:
+            raise ValueError(f"gated_dense: 8-bit weights need widths that are multiples of 16, got {self.hidden} and {self.inner}")
+        if not self.reads_fp8:
+            self.w_gate_up, self.w_down = quantize_weight(self.w_gate_up), quantize_weight(self.w_down)
+
+    @property
+    def reads_fp8(self) -> bool:
+        return isinstance(self.w_down, Fp8Weight)
+
+    def _forward_fp8(self, x, ctx):
+        gate_up = linear_fp8(x, self.w_gate_up, ctx.dtype, ctx)
+        act = empty_fp8_rows(gate_up.shape[0], self.inner, gate_up.device)
+        kernels.glu_act_fp8(gate_up, act.q, act.scales, bias=self.b_gate_up, limit=self.limit, alpha=self.alpha, kind=self.KINDS[self.activation])
+        y = linear_fp8(act, self.w_down, torch.float32, ctx)
+        return Addends(y, bias=self.b_down) if self.biases else y
+
     def forward(self, x, ctx):
+        if self.reads_fp8:
+            return self._forward_fp8(x, ctx)
         T = x.shape[0]
         if self.activation == "silu" and not self.biases:
             act = linear_silu(x, self.w_gate_up, ctx)

@@ -5,6 +5,8 @@ from __future__ import annotations
 import torch
 
 from .. import kernels
+from ..fp8 import Fp8Rows, empty_rows as empty_fp8_rows
+from ..matmul import empty_rows
 from .base import Addends, Norm, NormedPending, StreamCopy, StreamsPending, TensorSpec, register
 from .conv import ResidualShortConv
 
@@ -52,9 +54,29 @@ class RMSNorm(Norm):
         y, mix, out_w, mult = (pending.y, pending.mix, pending.out_w, pending.mult) if pending is not None else (None, None, None, 0.0)
         kernels.streams_mix_rmsnorm(x, y, mix, out_w, mult, read_w, self.weight, self.eps, out, rows=rows, store=store)
 
+    def _forward_fp8(self, h, delta, out: Fp8Rows, rows, store_h: bool) -> None:
+        """``forward`` into 8-bit rows: in one launch where the addends are one tensor (normed first or not), else through float32 rows."""
+        pending = delta.addends if isinstance(delta, NormedPending) and isinstance(delta.norm, RMSNorm) else None
+        y, gain, y_eps = delta, None, 0.0
+        if pending is not None:
+            y, gain, y_eps = pending.y, delta.norm.weight, delta.norm.eps
+        plain = (y is None or isinstance(y, torch.Tensor)) and self.groups == 1 and h.dim() == 2 and (rows is None or y is None or not store_h)
+        if pending is not None:
+            plain = (plain and delta.norm.groups == 1 and pending.scale == 1.0 and pending.bias is None and pending.extra is None
+                     and not pending.branch_normed)
+        if plain:
+            kernels.add_rmsnorm_fp8(h, y, self.weight, self.eps, out.q, out.scales, rows=rows, store_h=store_h, delta_gain=gain, delta_eps=y_eps)
+            return
+        normed = torch.empty(out.shape, dtype=torch.float32, device=h.device)
+        self.forward(h, delta, normed, rows=rows, store_h=store_h)
+        kernels.rows_to_fp8(normed, out.q, out.scales)
+
     def forward(self, h, delta, out, rows=None, store_h=True):
         if isinstance(delta, StreamCopy):
             delta = None                # nothing is pending; the copy that came with the stream is not needed here
+        if isinstance(out, Fp8Rows):
+            self._forward_fp8(h, delta, out, rows, store_h)
+            return
         if h.dim() == 3 or isinstance(delta, StreamsPending):
             # several residual streams: whoever asks for the plain norm (the output head) reads their sum
             self.forward_streams(h, delta, None, out, rows=rows, store=store_h)
@@ -115,6 +137,14 @@ def add_sum(h, a: Addends, out, weight=None, groups: int = 1, eps: float = 0.0, 
                                extra_scale=a.extra_scale, extra_bias=a.extra_bias, extra_gain=a.extra_gain,
                                branch_eps=a.branch_eps, weight=weight, weight_groups=groups, eps=eps, out=out, rows=rows,
                                store_h=store_h)
+
+
+def rows_for(reader, norm, h, width: int, dtype) -> torch.Tensor | Fp8Rows:
+    """What ``norm`` writes for the part ``reader``: 8-bit rows where the one reads and the other writes them (this very class of norm: one made
+    from it may have a ``forward`` of its own), else rows of the activation dtype."""
+    if getattr(reader, "reads_fp8", False) and type(norm) is RMSNorm:
+        return empty_fp8_rows(h.shape[0], width, h.device)
+    return empty_rows(h.shape[0], width, dtype=dtype, device=h.device)
 
 
 @register("norm", "none")
