@@ -299,7 +299,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 //                512 of its products, so two take the k blocks in turn.  (One issuer, N = 256, two accumulators: 984 cycles a k block, of which
 //                the tensor cores worked 512.)  The number of stages is even, so that a stage and an accumulator belong to one issuer, which
 //                waits for every phase of their barriers in order.
-//   warps 4-11 : a TMEM lane quadrant and 64 columns (a pair: 128) each: add, then store.  They hold up to 128 sums a thread, more registers than
+//   warps 4-11 : a TMEM lane quadrant and 64 columns (a pair: 128) each: add, then store. They hold up to 128 sums a thread, more registers than
 //                a block of 384 threads can give every one, so the other warps hand some of theirs over; what all have then is at most
 //                what the block was launched with.
 // Pairs walk over the tiles (a block an SM), so that the copies of the next tile run under the stores of the last; a block of a cut product has one.
@@ -308,9 +308,8 @@ constexpr int L8_REGS_ADD = 224, L8_REGS_OTHER = 56, L8_REGS_LAUNCH = 168, L8_GR
 static_assert(256 * L8_REGS_ADD + 128 * L8_REGS_OTHER <= L8_THREADS * L8_REGS_LAUNCH, "registers of the launch");
 constexpr int L8_BOX = 32 * 128;            // bytes of a warp's staged part of the output: 32 rows of 128 bytes
 constexpr uint32_t L8_STAGE = 2 * L8_A;     // 128 tokens and 128 weight rows
-
 struct L8Big {
-  uint64_t full[8], empty[8], acc_full[2][2], acc_empty[2][2];      // [half][turn]
+  uint64_t full[8], empty[8], acc_full[2][4], acc_empty[2][4];      // [half][accumulator]
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -327,8 +326,8 @@ __global__ void __launch_bounds__(L8_THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
                   LinearFp8 a, int boxes) {
   qb_follow();
-  constexpr int SIDE = PAIR ? 256 : 128, HALVES = PAIR ? 2 : 1, COLS = PAIR ? 128 : 64;
-  constexpr uint32_t TMEM = HALVES * 256;
+  constexpr int SIDE = PAIR ? 256 : 128, HALVES = PAIR ? 2 : 1, ACC = 4 / HALVES, COLS = PAIR ? 128 : 64;      // ACC: accumulators a half
+  constexpr uint32_t TMEM = 512;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   __shared__ L8Big sh;
@@ -352,8 +351,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       mbar_init(smem_u32(&sh.empty[s]), 1);
     }
     for (int s = 0; s < 4; ++s) {
-      mbar_init(smem_u32(&sh.acc_full[s >> 1][s & 1]), 1);
-      mbar_init(smem_u32(&sh.acc_empty[s >> 1][s & 1]), 8);      // the warps that add: a half's four of each block of a pair
+      mbar_init(smem_u32(&sh.acc_full[s / ACC][s % ACC]), 1);
+      mbar_init(smem_u32(&sh.acc_empty[s / ACC][s % ACC]), 8);      // the warps that add it: a half's four of each block of a pair
     }
     sh.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -420,15 +419,16 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
   } else if (warp < 3) {
     if (lane == 0 && (rank == 0 || !PAIR)) {
-      const uint32_t idesc = umma_idesc_e4m3(PAIR ? 256 : 128, 128), buf = (uint32_t)warp - 1u;
+      const uint32_t idesc = umma_idesc_e4m3(PAIR ? 256 : 128, 128), first = (uint32_t)warp - 1u;
       const uint64_t a_first = umma_desc_sw128(smem_u32(tiles)), b_first = umma_desc_sw128(smem_u32(tiles) + L8_A);
       const int mine = tile_first < tiles_all ? (tiles_all - tile_first + tile_step - 1) / tile_step : 0;
       const int turns = mine * k_blocks;
       uint32_t full_parity = 0u, empty_parity = 1u;
-      int s = (int)buf;
+      int s = (int)first;
+      uint32_t buf = first;
       bool ok = true;
 #pragma unroll 1
-      for (int turn = (int)buf; turn < turns && ok; turn += 2) {
+      for (int turn = (int)first; turn < turns && ok; turn += 2) {
         ok = mbar_wait(smem_u32(&sh.full[s]), full_parity, abort_flag);
         const uint64_t a_desc = a_first + (uint64_t)(s * (int)(L8_STAGE >> 4)), b_desc = b_first + (uint64_t)(s * (int)(L8_STAGE >> 4));
 #pragma unroll
@@ -436,7 +436,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           ok = ok && mbar_wait(smem_u32(&sh.acc_empty[h][buf]), empty_parity, abort_flag);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t to = tmem_base + (uint32_t)(h * 2 + (int)buf) * 128u;
+          const uint32_t to = tmem_base + ((uint32_t)(h * ACC) + buf) * 128u;
 #pragma unroll
           for (int k = 0; k < L8_BK / 32; ++k) {      // 32 bytes further along the swizzled row: +2 in the 16-byte address field
             // (a pair's half: 64 weight rows of each block)
@@ -447,7 +447,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
         if (!ok) break;
         if (PAIR) umma_commit_pair(smem_u32(&sh.empty[s])); else umma_commit(smem_u32(&sh.empty[s]));
-        empty_parity ^= 1u;
+        if ((buf += 2u) >= ACC) { buf = first; empty_parity ^= 1u; }
         if ((s += 2) >= a.stages) { s -= a.stages; full_parity ^= 1u; }
       }
     }
@@ -457,7 +457,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     const int quad = warp & 3, group = (warp - L8_FIRST) / 4, h = PAIR ? group : 0;
     // column i of the warp's sums: weight row n0 + col0 + i / 64 * 128 + i % 64
     const int col0 = group * 64;
-    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(PAIR ? h * 256 : group * 64);
+    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(PAIR ? h * ACC * 128 : group * 64);
     const uint32_t full0 = smem_u32(&sh.acc_full[h][0]), empty0 = PAIR ? mapa_u32(smem_u32(&sh.acc_empty[h][0]), 0u) : smem_u32(&sh.acc_empty[h][0]);
     const uint32_t staged = smem_u32(tiles) + (uint32_t)a.stages * L8_STAGE + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
     float x_ahead[AHEAD], w_ahead[WS][AHEAD];
@@ -494,18 +494,19 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         for (int d = 0; d < AHEAD; ++d) {
           const int kb = k0 + d;
           if (kb >= k_blocks || !ok) break;
-          const uint32_t buf = turn & 1u, at = from + buf * 128u;
+          const uint32_t buf = turn % ACC, at = from + buf * 128u;
           float f[WS];
 #pragma unroll
           for (int i = 0; i < WS; ++i) f[i] = x_ahead[d] * w_ahead[i][d];
           if (kb + AHEAD < k_blocks) {
-            if (has_x) x_ahead[d] = xs[(size_t)(kb + AHEAD) * a.T];
+            const int next = kb + AHEAD;
+            if (has_x) x_ahead[d] = xs[(size_t)next * a.T];
 #pragma unroll
             for (int i = 0; i < WS; ++i)
-              if (has_w[i]) w_ahead[i][d] = ws[i * a.blocks + kb + AHEAD];
+              if (has_w[i]) w_ahead[i][d] = ws[i * a.blocks + next];
           }
           // tcgen05.ld is .sync.aligned: the lanes vote on the wait's answer
-          ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * buf, turn >> 1 & 1u, abort_flag) ? 1 : 0) != 0;
+          ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * buf, turn / ACC & 1u, abort_flag) ? 1 : 0) != 0;
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           uint32_t v[2][16];
@@ -704,9 +705,10 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
     QB_LAUNCH_CHECK();
     return 0;
   }
-  // pairs of blocks where their tiles give every SM two turns or more, else tiles of 128 x 128, cut along k where they are few
-  const long long pair_tiles = (long long)((T + 255) / 256) * ((N + 255) / 256);
-  const bool pair = pair_tiles >= sms;
+  // Pairs of blocks where tiles of 128 x 128 would be more than one for every SM (768 tokens, 4,096 x 4,096: 20 us, 29 with single blocks; 512, one tile an
+  // SM: 20 and 15), but for tokens that fill half a pair's tile at most; else single blocks, cut along k where they are few.
+  const long long singles = (long long)((T + 127) / 128) * ((N + 127) / 128);
+  const bool pair = T > 128 && singles > sms;
   const int width = pair ? 256 : 128;
   const size_t size = out_dtype == QB_F32 ? 4 : 2;
   const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
@@ -719,8 +721,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
   const size_t stage = 2 * L8_A, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;
   a.stages = a.cut > 1 ? 6 : 4;
-  const size_t ring = stage * a.stages, need = a.cut > 1 ? (size_t)128 * (128 + 4) * 4 : 0;
-  const size_t smem = (ring > need ? ring : need) + staged + 1024;
+  const size_t smem = stage * a.stages + staged + 1024;
   rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, 128, bytes);
   if (!rc) rc = l8_map(&tm_x, x, (uint64_t)T, (uint64_t)K, 1, 128, bytes);
   if (!rc && boxes)
