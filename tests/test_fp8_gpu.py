@@ -286,3 +286,37 @@ def test_on_another_stream_and_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("T,K,N", [(3, 2048, 640), (24, 2048, 640), (50, 2048, 640), (200, 2048, 640), (700, 1024, 5000)])
+def test_two_calls_at_once(T, K, N):
+    """On two streams, neither waiting for the other: no call leaves anything that another could read."""
+    from quanta_b200 import kernels
+    a, b = _operands(T, K, N, 1), _operands(T, K, N, 2)
+    want = []
+    for ops in (a, b):
+        want.append(torch.empty(T, N, device=DEV))
+        kernels.linear_fp8(*ops, want[-1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.empty(T, N, device=DEV) for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for k, ops in enumerate((a, b)):
+            with torch.cuda.stream(streams[k]):
+                kernels.linear_fp8(*ops, outs[k][i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[k]) for k in range(2) for o in outs[k])
+
+
+def test_empty_calls():
+    from quanta_b200 import kernels
+    q, s = _empty_rows(0, 256)
+    kernels.rows_to_fp8(torch.empty(0, 256, device=DEV), q, s)
+    kernels.glu_act_fp8(torch.empty(0, 512, device=DEV), q, s)
+    kernels.add_rmsnorm_fp8(torch.empty(0, 256, device=DEV), None, torch.ones(256, device=DEV), 1e-5, q, s)
+    _, _, w, ws = _operands(1, 256, 100, 1)
+    kernels.linear_fp8(q, s, w, ws, torch.empty(0, 100, device=DEV))
+    x, xs, _, _ = _operands(5, 256, 100, 1)
+    kernels.linear_fp8(x, xs, w[:0], ws[:0], torch.empty(5, 0, device=DEV))
+    torch.cuda.synchronize()

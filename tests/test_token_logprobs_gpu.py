@@ -73,6 +73,23 @@ def test_scores(n, V, top, dtype):
     assert all(torch.equal(a, b) for a, b in zip(_scores(x, t, top), _scores(x, t, top)))
 
 
+@pytest.mark.parametrize("n,V,dtype", [(1, 4300037, torch.float32), (1, 9000001, torch.bfloat16), (1190, 262150, torch.float32), (1190, 530001, torch.bfloat16), (700, 4097, torch.float32),
+                                       (90, 33333, torch.bfloat16)])
+def test_long_rows_and_many(n, V, dtype):
+    """Rows longer than a block keeps a maximum of every 512 bytes for, and numbers of rows that are cut in three, five and more parts."""
+    g = _gen(V)
+    x = torch.randn(n, V, device=DEV, generator=g, dtype=dtype)
+    t = torch.randint(0, V, (n,), device=DEV, generator=g).to(torch.int32)
+    lp, en, ids, best = _scores(x, t, 20)
+    for r in sorted({0, n // 2, n - 1}):
+        _check(x[r: r + 1], t[r: r + 1].contiguous(), 20)
+        lse = torch.logsumexp(x[r].double(), 0)
+        order = _order(x[r: r + 1].double(), 20)[0]
+        assert torch.equal(ids[r], order)
+        assert torch.all((best[r].double() - (x[r].double()[order.long()] - lse)).abs() < 1e-4) and abs(float(lp[r]) - float(x[r, int(t[r])].double() - lse)) < 1e-4
+    assert bool(torch.isfinite(lp).all()) and bool(torch.isfinite(en).all()) and bool((best[:, :-1] >= best[:, 1:]).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n", [1, 40, 200])
 def test_ties_masks_and_uneven_rows(n, dtype):
