@@ -21,6 +21,7 @@ namespace {
 
 constexpr int TL_MAX_WARPS = 16, TL_GROUPS = 128, TL_CAND = 1024, TL_MAX_TOP = 64, TL_MAX_CUT = 16, TL_SLOTS = 2048;
 constexpr float TL_LOG2E = 1.4426950408889634f;
+constexpr float TL_LOW = -3.2964854295465914e+38f;      // near the lowest numbers, and a bfloat16
 
 struct TokenLogprobs {
   const void* logits;
@@ -90,7 +91,8 @@ __device__ __forceinline__ TlSum tl_join(TlSum v) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float d = v.m - m;
-  if (d > -INFINITY) {      // (NaN where both are infinite)
+  if (v.m <= TL_LOW) v.u = 0.f * v.s;
+  if (d >= -200.f) {      // (NaN where both are infinite)
     const float f = tl_exp2(d * TL_LOG2E);
     v.u = (v.u + v.s * d) * f;
     v.s *= f;
@@ -146,8 +148,9 @@ template <typename T> struct TlRow {
     const uint32_t w = PER == 4 ? 0xff800000u : 0xff80ff80u;
     return make_uint4(w, w, w, w);
   }
-  // what lies so far below the maximum m that its weight is zero anyway, raised to where it still is: differences stay numbers
-  __device__ static float floor_of(float m) { return fmaxf(m - fmaxf(200.f, fabsf(m) * 0.015625f), -3.3e38f); }
+  // What lies so far below the maximum m that its weight is zero anyway is raised to where it still is: differences stay numbers.  Below TL_LOW
+  // there is no room for that; a -inf there leaves u without a number, which is zero then, all weights but those of m being zero (`tl_join`).
+  __device__ static float floor_of(float m) { return m <= TL_LOW ? -INFINITY : fmaxf(m - fmaxf(200.f, fabsf(m) * 0.015625f), TL_LOW); }
   __device__ static void numbers_above(const uint4& q, float least, float (&v)[PER]) {
     if constexpr (PER == 4) {
       numbers(q, v);
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(TokenLogprobs a
     }
     if (top > my_top) {
       const float d = my_top - top;
-      if (d == -INFINITY) {      // nothing yet, or a NaN that has to be seen
+      if (d < -200.f) {      // nothing yet, or nothing that still has a weight, or a NaN that has to be seen
         s2.x *= 0.f, s2.y *= 0.f;
         u2 = s2;
       } else {
@@ -497,7 +500,7 @@ extern "C" int qb_token_logprobs(const void* logits, int dtype, long long stride
   // Few rows: blocks of 512 threads, as many a row as there are SMs for.  More: blocks of 256, four an SM, which go through some 2,750 float32 or 3,900
   // bfloat16 numbers a microsecond and take 5 us behind their part (measured); a row is cut so that the waves of blocks take the least
   // (rows of 200,064: 150 rows 44 us in four parts, 34 in three; 300 rows 72 in two, 63 in five).  Rows for two waves or more are not cut.
-  const int threads = 5 * n < 3 * sms ? 512 : 256;
+  const int threads = 5ll * n < 3 * sms ? 512 : 256;
   if (threads == 512) {
     while (a.cut < TL_MAX_CUT && (long long)n * a.cut < sms && V / a.cut >= 4096) a.cut *= 2;
   } else if (n < 8 * sms) {

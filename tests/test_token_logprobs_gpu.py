@@ -187,3 +187,47 @@ def test_in_a_graph_and_on_another_stream():
         graph.replay()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [8, 200])
+def test_rows_of_the_lowest_numbers(n, dtype):
+    """Masks of the type's lowest value, alone, beside -inf (which is less probable), and beside numbers some steps above it.
+
+    Of the differences to the largest number only zeros have a weight, so the sum is exact: what is left are the logarithm (an ulp) and the roundings of
+    the differences."""
+    V, low = 20000, torch.finfo(dtype).min
+    g = _gen(n)
+    x = torch.randn(n, V, device=DEV, generator=g)
+    x[0] = low
+    x[1] = low
+    x[1, [17, 19990]] = 0.0
+    x[2] = -torch.inf
+    x[2, 100:1100] = low
+    x[3] = low
+    x[3, ::2] = -3.35e38
+    x[4, :19000] = low
+    x[5] = -torch.inf
+    x[5, :9000] = low
+    x[5, 19000:] = -3.0e38
+    x[6] = low
+    x[6, 5000] = torch.nan
+    x[7], x[7, 5:10] = low, -3.2965e38
+    x = x.to(dtype)
+    t = torch.full((n,), 4, dtype=torch.int32, device=DEV)
+    t[2] = 1099
+    lp, en, ids, best = _scores(x, t, 20)
+    assert torch.equal(ids, _order(x.double(), 20))
+    keep = torch.arange(n, device=DEV) != 6
+    assert bool(torch.isnan(lp[6])) and bool(torch.isnan(en[6])) and bool(torch.isnan(best[6]).all())
+    d = x[keep].double() - x[keep].double().amax(1, keepdim=True)
+    log_s = d.exp().sum(1).log()
+    tol = torch.full_like(log_s, 4 * U)
+    tol[4] = tol[7:] = 2.0 ** -21 + (V / 512 + 100) * U      # rows with ordinary numbers, as above
+    for got, want in ((lp[keep, None], d.gather(1, t[keep, None].long())), (best[keep], d.gather(1, ids[keep].long()))):
+        want = want - log_s[:, None]
+        assert torch.equal(torch.isinf(got), torch.isinf(want))
+        fine = torch.isfinite(want)
+        assert torch.all(((got.double() - want).abs() <= tol[:, None] * (8 + log_s[:, None]) + 4 * U * want.abs())[fine])
+    ent = torch.special.entr(torch.softmax(d, 1)).sum(1)
+    assert torch.all((en[keep].double() - ent).abs() <= tol * 16 * (1 + ent))
