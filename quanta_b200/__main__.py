@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import sys
 import tempfile
 
@@ -74,6 +75,13 @@ def _cmd_generate(a) -> int:
     return 0
 
 
+def _numbers(x):
+    """``x`` with None (null in JSON, which has no other word) for what is no finite number."""
+    if isinstance(x, (list, dict)):
+        return [_numbers(v) for v in x] if isinstance(x, list) else {k: _numbers(v) for k, v in x.items()}
+    return x if not isinstance(x, float) or math.isfinite(x) else None
+
+
 def _cmd_score(a) -> int:
     opened = _open(a)
     if opened is None:
@@ -83,7 +91,7 @@ def _cmd_score(a) -> int:
         line = {"tokens": len(text), "logprob": sum(s.logprobs), "perplexity": s.perplexity, "logprobs": s.logprobs, "entropies": s.entropies}
         if a.top:
             line |= {"top_ids": s.top_ids, "top_logprobs": s.top_logprobs}
-        print(json.dumps(line))
+        print(json.dumps(_numbers(line), allow_nan=False))
     if tmp is not None:
         tmp.cleanup()
     return 0
@@ -137,7 +145,7 @@ def main(argv=None) -> int:
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--stats", action="store_true", help="print run statistics to standard error")
     g.set_defaults(fn=_cmd_generate)
-    s = sub.add_parser("score", parents=[m], help="log probabilities of given token ids")
+    s = sub.add_parser("score", parents=[m], help="log probabilities of given token ids (null: minus infinity, or the perplexity of one token)")
     s.add_argument("--top", type=int, default=0, help="also the most probable tokens of every place")
     s.set_defaults(fn=_cmd_score)
     r = sub.add_parser("random-weights", help="write a model folder with seeded random weights")

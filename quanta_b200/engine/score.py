@@ -29,8 +29,13 @@ class TextScores:
 
     @property
     def perplexity(self) -> float:
-        """exp of the mean of -logprobs; NaN for a text of one token."""
-        return math.exp(-sum(self.logprobs) / len(self.logprobs)) if self.logprobs else math.nan
+        """exp of the mean of -logprobs (infinite where that is no float); NaN for a text of one token."""
+        if not self.logprobs:
+            return math.nan
+        try:
+            return math.exp(-sum(self.logprobs) / len(self.logprobs))
+        except OverflowError:
+            return math.inf
 
 
 def score_rows(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, status: torch.Tensor | None = None):

@@ -1258,6 +1258,7 @@ def glu_act(gate_up: torch.Tensor, out: torch.Tensor, *, bias=None, kind: int = 
 
 FP8_BLOCK = 128                 # columns of a row, and rows and columns of a weight, that share a scale
 E4M3 = torch.float8_e4m3fn
+MOST_ROWS = 1 << 30             # rows, and columns of a row: the kernels count them, and what they take together, in 32 bits
 
 
 _VOID, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
@@ -1296,9 +1297,15 @@ def _stream_of(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
+def _sizes(what: str, *sizes: int) -> None:
+    if max(sizes) > MOST_ROWS:
+        raise ValueError(f"{what}: sizes of at most {MOST_ROWS} are taken, got {max(sizes)}")
+
+
 def _fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, cols: int, name: str) -> None:
     _want(q, E4M3, name); _want(scales, torch.float32, f"the scales of {name}")
     blocks = -(-cols // FP8_BLOCK)
+    _sizes(what, n, cols)
     if tuple(q.shape) != (n, cols) or tuple(scales.shape) != (blocks, n):
         raise ValueError(f"{what}: {name} must be [{n}, {cols}] and its scales [{blocks}, {n}], got {tuple(q.shape)} and {tuple(scales.shape)}")
 
@@ -1325,6 +1332,7 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: torch.Tensor | None, weight: torch.T
         if delta is None or delta_gain.numel() != H:
             raise ValueError("add_rmsnorm_fp8: delta_gain needs a delta and H numbers")
     n = T if rows is None else rows.numel()
+    _sizes("add_rmsnorm_fp8", T, S)
     if rows is not None:
         _want(rows, torch.int32, "rows")
         if store_h and delta is not None:
@@ -1384,6 +1392,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("linear_fp8: x, w and out must be matrices")
     T, K = x.shape
     N = w.shape[0]
+    _sizes("linear_fp8", N)
     _fp8_rows("linear_fp8", x, x_scales, T, K, "x")
     if w.shape[1] != K or tuple(out.shape) != (T, N):
         raise ValueError(f"linear_fp8: w {tuple(w.shape)} and out {tuple(out.shape)} do not fit x {tuple(x.shape)}")
@@ -1415,6 +1424,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
     n, V = logits.shape
     if V == 0:
         raise ValueError("token_logprobs: an empty vocabulary")
+    _sizes("token_logprobs", n, V)
     if (logprob is None) != (tokens is None):
         raise ValueError("token_logprobs: logprob and tokens belong together")
     if (ids is None) != (best is None):

@@ -65,3 +65,23 @@ def test_scores():
             kernels.token_logprobs(**(ok | bad))
     with pytest.raises(ValueError, match="at most"):
         kernels.token_logprobs(torch.zeros(4, 3), None, None, None, ids[:, :4].contiguous(), best[:, :4].contiguous())
+
+
+def test_sizes_that_32_bits_do_not_count():
+    many = 2 ** 30 + 16
+    meta = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="at most"):
+        kernels.rows_to_fp8(meta(many, 16), meta(many, 16, dtype=E4M3), meta(1, many))
+    with pytest.raises(ValueError, match="at most"):
+        kernels.glu_act_fp8(meta(1, 2 * many), meta(1, many, dtype=E4M3), meta(many // 128 + 1, 1))
+    with pytest.raises(ValueError, match="at most"):
+        kernels.add_rmsnorm_fp8(meta(many, 16), None, meta(16), 1e-5, meta(many, 16, dtype=E4M3), meta(1, many))
+    with pytest.raises(ValueError, match="at most"):
+        kernels.add_rmsnorm_fp8(meta(2, 16), meta(2, many, 16), meta(16), 1e-5, meta(2, 16, dtype=E4M3), meta(1, 2))
+    with pytest.raises(ValueError, match="at most"):
+        kernels.linear_fp8(meta(1, 16, dtype=E4M3), meta(1, 1), meta(many, 16, dtype=E4M3), meta(many // 128 + 1, 1), meta(1, many))
+    with pytest.raises(ValueError, match="at most"):
+        kernels.linear_fp8(meta(many, 16, dtype=E4M3), meta(1, many), meta(16, 16, dtype=E4M3), meta(1, 1), meta(many, 16))
+    for n, V in ((many, 1), (1, 2 ** 32 + 5)):
+        with pytest.raises(ValueError, match="at most"):
+            kernels.token_logprobs(meta(n, V), None, None, meta(n))
