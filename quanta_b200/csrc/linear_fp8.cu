@@ -2,16 +2,22 @@
 // of a row of x and for every 128 x 128 block of w, on the 5th-generation tensor cores.
 //
 // The scales change every 128 k, so what the tensor cores sum over one block of k is taken out of TMEM, scaled and added in float32 registers
-// (one rounding a block); two accumulators take turns, so that the tensor cores work on the next block meanwhile.  That addition has as
-// many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the two forms:
+// (one rounding a block); several accumulators take turns, so that the tensor cores work on the next block meanwhile.  That addition has as
+// many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the forms:
 //
-//  * up to 64 tokens (linear_fp8_few_kernel; up to 16 linear_fp8_few.cu, mostly): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
+//  * 8 tokens or fewer, and more where the matrix is small: linear_fp8_few.cu, without tensor memory (its rule and both sides' times stand there).
+//  * up to 64 tokens (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
 //    height of the MMA and the weights are read once.  A TMEM lane is a weight row, a column a token; the columns' scales come from shared memory.
 //  * more (linear_fp8_kernel): the tokens are the rows, the weights the columns.  A lane has its token's scale in a register and one weight
 //    scale for all of its columns, so the addition is one packed multiply-add for two numbers and reads nothing.  (With the tokens as columns the
 //    scales' way from shared memory to the registers, 128 KB a k block of 256 tokens, took 1,024 cycles: 8,192 x 4,096 x 22,016 1,175 us.)
 //    Steps of many tokens: two blocks on neighbouring SMs take 256 tokens x 256 weight rows together (cta_group::2), each fetching its own 128
 //    tokens and half of the weight tile.
+//
+// Measured on a B200, one product after another in a graph: 8,192 tokens, 4,096 x 22,016 650 to 680 us (2.2 PFLOP/s; 775 where products follow one another
+// for seconds and the clock falls under the power limit), which is the power limit's and the issue's, the tensor cores being active 64% of the
+// cycles; 1,024 x 4,096 x 4,096 20 us; 317 x 5,648 x 2,000 16.6 us and 512 x 4,096 x 4,096 15 us, single blocks, which are bound by what an SM takes from
+// L2 (some 50 bytes a cycle; a 128 x 128 tile reads 256 bytes for every 128 x 128 products); 32 tokens, 4,096 x 11,008 14 us, the bytes 7.
 //
 // A product of few tiles is cut along k over the blocks of a cluster; each leaves its sums in shared memory, and every block adds one share of
 // them, the blocks' parts in order, so the result is the same in every run.
@@ -25,7 +31,8 @@ namespace {
 
 constexpr int L8_M = 128, L8_BK = 128;      // weight rows of a tile; k of a stage: 128 bytes, one swizzle row
 constexpr int L8_A = L8_M * L8_BK;          // bytes of a weight tile
-constexpr int L8_MAX_STAGES = 12, L8_SCALES = 4, L8_AHEAD = 3;      // slots of the scales' ring, blocks they are fetched ahead of it
+constexpr int L8_MAX_STAGES = 8;
+constexpr int L8_SCALES = 4, L8_AHEAD = 3;      // slots of the scales' ring, blocks they are fetched ahead of it
 constexpr int L8_FIRST = 4;                 // the first adding warp
 constexpr int L8_FEW_THREADS = 256, L8_THREADS = 384;
 
@@ -36,10 +43,11 @@ struct LinearFp8 {
   int blocks, per;            // k blocks, k blocks a block of the cluster takes
   int stages, cut, t_tiles;
   int* status;
+  int early;
 };
 
 struct L8Shared {
-  uint64_t full[L8_MAX_STAGES], empty[L8_MAX_STAGES], acc_full[2], acc_empty[2], sc_full[L8_SCALES], sc_empty[L8_SCALES];
+  uint64_t full[L8_MAX_STAGES], acc_full[L8_MAX_STAGES], acc_empty[L8_MAX_STAGES], sc_full[L8_SCALES], sc_empty[L8_SCALES];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -92,17 +100,18 @@ __device__ __forceinline__ void l8_store4(O* row, int n, int N, float4 v) {
 }
 
 //   warp 0     : TMA producer: per k block the weight tile [128 x 128] and the token tile [NT x 128], 128-byte swizzle, into a ring of stages
-//   warp 1     : MMA issuer: 4 x tcgen05.mma (32 k each) a stage; commits free the stage and hand the accumulator over
+//   warp 1     : MMA issuer: 4 x tcgen05.mma (32 k each) a stage; the commit hands the accumulator over and frees the stage
 //   warp 2     : scales: xs[b, t] * ws[n / 128, b] of the tile's tokens into a ring in shared memory, fetched several blocks ahead
 //   warps 4-7  : one TMEM lane quadrant each: add, then store
 // NT: tokens of a tile (the MMA's N)
 template <int NT, typename O>
 __global__ void __launch_bounds__(L8_FEW_THREADS)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, LinearFp8 a) {
-  qb_follow();
+  if (!a.early) qb_follow();
   constexpr int ADDERS = 4, COLS = NT;
   constexpr uint32_t STAGE = L8_A + NT * L8_BK;
-  constexpr uint32_t TMEM = 2 * NT < 32 ? 32 : 2 * NT;
+  constexpr int ACC = NT <= 32 ? 8 : 4;
+  constexpr uint32_t TMEM = ACC * NT;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   __shared__ L8Shared sh;
@@ -112,13 +121,12 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   const int n0 = tile / a.t_tiles * L8_M, t0 = tile % a.t_tiles * NT;
   const int k_first = rank * a.per, k_blocks = max(0, min(a.per, a.blocks - k_first));
   volatile int* abort_flag = &sh.abort_flag;
+  // weights that one token tile reads leave L2 first; tokens, and weights that others read too, stay
+  const uint64_t pol_w = a.t_tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first(), pol_x = l2_policy_evict_last();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_u32(&sh.full[s]), 1);
-      mbar_init(smem_u32(&sh.empty[s]), 1);
-    }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < a.stages; ++s) mbar_init(smem_u32(&sh.full[s]), 1);
+    for (int s = 0; s < ACC; ++s) {
       mbar_init(smem_u32(&sh.acc_full[s]), 1);
       mbar_init(smem_u32(&sh.acc_empty[s]), ADDERS);
     }
@@ -128,7 +136,14 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     sh.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the first weights may be asked for before the launch ahead has ended; its tokens are not there yet
+    for (int kb = 0; a.early && kb < min(a.stages, k_blocks); ++kb) {
+      mbar_expect_tx(smem_u32(&sh.full[kb]), STAGE);
+      tma_load_2d(smem_u32(tiles) + (uint32_t)kb * STAGE, &tm_w, (k_first + kb) * L8_BK, n0, smem_u32(&sh.full[kb]), pol_w);
+    }
   }
+  // (no tensor memory before it: a block of the launch ahead may still have to get its own)
+  if (a.early) qb_follow();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -142,19 +157,25 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 
   if (warp == 0) {
     if (lane == 0) {
-      // weights that one token tile reads leave L2 first; tokens, and weights that others read too, stay
-      const uint64_t pol_w = a.t_tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      uint32_t parity = 1u;
       int s = 0, armed = 0;
 #pragma unroll 1
       for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!mbar_wait(smem_u32(&sh.empty[s]), parity, abort_flag)) break;
+        // a stage is free when the products of the k block that it held are there (no more stages than accumulators: their barrier is then at that phase)
+        const int past = kb - a.stages;
+        if (past >= 0 && !mbar_wait(smem_u32(&sh.acc_full[past % ACC]), (uint32_t)(past / ACC) & 1u, abort_flag)) break;
         const uint32_t full = smem_u32(&sh.full[s]), st = smem_u32(tiles) + (uint32_t)s * STAGE;
-        mbar_expect_tx(full, STAGE);
-        tma_load_2d(st, &tm_w, (k_first + kb) * L8_BK, n0, full, pol_w);
+        if (!a.early || kb >= a.stages) {
+          mbar_expect_tx(full, STAGE);
+          tma_load_2d(st, &tm_w, (k_first + kb) * L8_BK, n0, full, pol_w);
+        }
         tma_load_2d(st + L8_A, &tm_x, (k_first + kb) * L8_BK, t0, full, pol_x);
         armed = kb + 1;
-        if (++s == a.stages) { s = 0; parity ^= 1u; }
+        if (++s == a.stages) s = 0;
+      }
+      if (*abort_flag && a.early && armed < min(a.stages, k_blocks)) {
+        // weights are on their way whose tokens were not asked for, so that their barriers do not complete: give them time
+        const uint64_t since = global_ns();
+        for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
       }
       if (*abort_flag) {
         // let the copies that were issued land before this block's shared memory is given away
@@ -172,8 +193,8 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       int s = 0;
 #pragma unroll 1
       for (int kb = 0; kb < k_blocks; ++kb) {
-        const int half = kb & 1;
-        if (!mbar_wait(smem_u32(&sh.acc_empty[half]), (uint32_t)(kb >> 1 & 1) ^ 1u, abort_flag)) break;
+        const int half = kb % ACC;
+        if (!mbar_wait(smem_u32(&sh.acc_empty[half]), (uint32_t)(kb / ACC & 1) ^ 1u, abort_flag)) break;
         if (!mbar_wait(smem_u32(&sh.full[s]), parity, abort_flag)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t st = smem_u32(tiles) + (uint32_t)s * STAGE;
@@ -181,7 +202,6 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 #pragma unroll
         for (int k = 0; k < L8_BK / 32; ++k)      // 32 bytes further along the swizzled row: +2 in the 16-byte address field
           umma_e4m3(tmem_base + (uint32_t)(half * NT), a_desc + 2 * k, b_desc + 2 * k, idesc, k != 0);
-        umma_commit(smem_u32(&sh.empty[s]));
         umma_commit(smem_u32(&sh.acc_full[half]));
         if (++s == a.stages) { s = 0; parity ^= 1u; }
       }
@@ -226,10 +246,10 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     bool ok = true;
 #pragma unroll 1
     for (int kb = 0; kb < k_blocks; ++kb) {
-      const int half = kb & 1, slot = kb % L8_SCALES;
+      const int half = kb % ACC, slot = kb % L8_SCALES;
       // tcgen05.ld is .sync.aligned: the lanes vote on the waits' answers
       ok = mbar_wait(smem_u32(&sh.sc_full[slot]), (uint32_t)(kb / L8_SCALES & 1), abort_flag);
-      ok = ok && mbar_wait(smem_u32(&sh.acc_full[half]), (uint32_t)(kb >> 1 & 1), abort_flag);
+      ok = ok && mbar_wait(smem_u32(&sh.acc_full[half]), (uint32_t)(kb / ACC & 1), abort_flag);
       ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -661,20 +681,23 @@ int l8_many(CUtensorMap& tm_w, CUtensorMap& tm_x, CUtensorMap& tm_out, LinearFp8
 }  // namespace
 
 // linear_fp8_few.cu
-bool qb_linear_fp8_tokens_takes(int T, int K, int N, int sms);
-int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int sms,
-                         cudaStream_t stream);
+bool qb_linear_fp8_tokens_takes(int T, int K, int N);
+int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int early,
+                         int sms, cudaStream_t stream);
 
+// early: w and ws were written two launches before this one at the latest (or by the host); the kernels for few tokens then ask for their
+// first pieces before the launch ahead has ended.
 extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N,
-                             int* status, cudaStream_t stream) {
+                             int early, int* status, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return QB_ERR_BAD_ARG;
   if (out_dtype != QB_F32 && out_dtype != QB_BF16) return QB_ERR_BAD_ARG;
   int sms = 0;
   int rc = sm_count(sms);
   if (rc) return rc;
-  if (qb_linear_fp8_tokens_takes(T, K, N, sms)) return qb_linear_fp8_tokens(x, xs, w, ws, out, out_dtype, T, K, N, sms, stream);
+  if (qb_linear_fp8_tokens_takes(T, K, N)) return qb_linear_fp8_tokens(x, xs, w, ws, out, out_dtype, T, K, N, early, sms, stream);
   LinearFp8 a{xs, ws, out, T, K, N};
+  a.early = early;
   a.blocks = (K + L8_BK - 1) / L8_BK;
   a.status = status;
   const CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -688,7 +711,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
     a.per = (a.blocks + a.cut - 1) / a.cut;
     const size_t stage = L8_A + (size_t)NT * L8_BK, need = a.cut > 1 ? (size_t)NT * L8_M * 4 : 0;
     int stages = (int)(100 * 1024 / stage);
-    if (stages > L8_MAX_STAGES) stages = L8_MAX_STAGES;
+    if (stages > (NT <= 32 ? 8 : 4)) stages = NT <= 32 ? 8 : 4;      // (accumulators)
     if (stages > a.per) stages = a.per;
     a.stages = stages;
     const size_t ring = stage * stages, smem = (ring > need ? ring : need) + 1024;

@@ -1,4 +1,4 @@
-// The product of linear_fp8.cu for at most 16 tokens, of a small matrix 32: bound by the bytes of w, and by what a launch costs besides them.
+// The product of linear_fp8.cu for few tokens, of a small matrix for more: bound by the bytes of w, and by what a launch costs besides them.
 //
 // A block takes 16 rows of w, its warps blocks of 128 k (one scale each) in turn.  A lane loads the 32 numbers of a row's 128 that it
 // then multiplies (the order of k inside an mma is free as long as both operands have it), 32 bytes a load, so that weights go from memory to
@@ -6,23 +6,27 @@
 // float32, the sum is scaled by token and weight block and added in float32; the warps' parts are added in the order of the warps, so a
 // row's bits are the same in every step of as many warps a block.
 //
-// Measured on a B200, one product after another in a graph, weights from memory, microseconds (bytes at 6.5 TB/s / this / tcgen05): one token,
-// 4,096 x 22,016 13.8 / 18.2 / 18.3, 2,048 x 2,048 0.6 / 2.1 / 5.5; 8 tokens, 2,048 x 11,264 3.5 / 7.2 / 8.7, 5,632 x 2,048 1.8 / 4.5 / 7.5; 16 tokens,
-// 5,632 x 2,048 1.8 / 5.4 / 7.5, 4,096 x 22,016 13.8 / 21.3 / 19.3; 32 tokens, 2,048 x 2,048 0.6 / 3.9 / 6.2, 2,048 x 11,264 3.5 / 13 / 10.5.  What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps
-// and a cluster's parts before and behind the bytes; what bounds this one in a large matrix is the issue of instructions (154 a warp for 2 KB:
-// e4m3 operands of mma.sync are converted to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took
-// the same time; four pieces ahead instead of two a longer one (fewer warps).
+// Measured on a B200, one product after another in a graph, weights from memory, microseconds (bytes at 6.5 TB/s / this / tcgen05):
+//   one token    4,096 x 22,016 13.8 / 18.5 / 18.6, 2,048 x 2,048 0.6 / 2.1 / 5.5
+//   8 tokens     2,048 x 11,264 3.5 / 7.2 / 8.7, 5,632 x 2,048 1.8 / 4.5 / 7.5
+//   16           5,632 x 2,048 1.8 / 5.4 / 7.5, 4,096 x 22,016 13.8 / 21.3 / 18.8
+//   32           2,048 x 2,048 0.6 / 3.4 / 6.0, 5,632 x 2,048 1.8 / 7.1 / 8.5, 4,096 x 4,096 2.6 / 10.7 / 8.9, 2,048 x 11,264 3.5 / 13 / 10.4
+//   64           1,024 x 1,024 0.2 / 2.4 / 5.8, 2,048 x 2,048 0.6 / 6.0 / 7.5, 2,048 x 4,096 1.3 / 10.9 / 9.4
+//   96           2,048 x 2,048 0.6 / 8.6 / 7.7;   128: 2,048 x 768 0.2 / 5.1 / 8.0;   256: 1,024 x 1,024 0.2 / 7.3 / 7.6, 2,048 x 768 0.2 / 8.9 / 8.1
+// What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps and a cluster's parts before and behind the bytes; what bounds
+// this one in a large matrix or with many tokens is the issue of instructions (154 a warp for 2 KB and 8 tokens: e4m3 operands of mma.sync are converted
+// to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took the same time; four pieces ahead instead of two a
+// longer one (fewer warps).  Weights asked for before the launch ahead has ended (`early`): norm, product, activation and product of 4,096 x 11,008 for
+// one token 33.0 -> 32.2 us, for 32 38.1 -> 35.8, of 2,048 x 5,632 15.0 -> 13.7 and 22.5 -> 21.1.
 #include "fp8.cuh"
 
 namespace {
-
-
 
 struct LinearFp8Few {
   const uint8_t *x, *w;
   const float *xs, *ws;
   void* out;
-  int T, K, N, blocks;
+  int T, K, N, blocks, early;
 };
 struct alignas(16) L8Piece {
   uint32_t u[8];
@@ -61,15 +65,15 @@ __device__ __forceinline__ void l8f_mma(float (&c)[4], uint32_t a0, uint32_t a1,
 template <int NT, int D, int XD, int WARPS, int MINB, bool WIDE, typename O>
 __global__ void __launch_bounds__(WARPS * 32, MINB) linear_fp8_tokens_kernel(LinearFp8Few a) {
   static_assert(D % XD == 0, "the ring of x divides the ring of w");
-  qb_follow();
+  if (!a.early) qb_follow();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16, t0 = blockIdx.y * NT * 8;
   const uint8_t* wr[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) wr[h] = a.w + (size_t)min(n0 + h * 8 + g, a.N - 1) * a.K + t * 32;
   const uint8_t* xr[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) xr[n] = a.x + (size_t)min(n * 8 + g, a.T - 1) * a.K + t * 32;
+  for (int n = 0; n < NT; ++n) xr[n] = a.x + (size_t)min(t0 + n * 8 + g, a.T - 1) * a.K + t * 32;
   const float* ws = a.ws + (size_t)(n0 / FP8_BLOCK) * a.blocks;
   L8Piece wb[D][2], xb[XD][NT];
   float xsb[XD][NT][2], wsb[XD];
@@ -85,12 +89,13 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) linear_fp8_tokens_kernel(Lin
       xb[at][n] = l8f_load<WIDE, false>(xr[n] + kb * FP8_BLOCK, left);
       // the scales of the tokens whose sums this lane has
 #pragma unroll
-      for (int i = 0; i < 2; ++i) xsb[at][n][i] = kb < a.blocks ? a.xs[(size_t)kb * a.T + min(n * 8 + 2 * t + i, a.T - 1)] : 0.f;
+      for (int i = 0; i < 2; ++i) xsb[at][n][i] = kb < a.blocks ? a.xs[(size_t)kb * a.T + min(t0 + n * 8 + 2 * t + i, a.T - 1)] : 0.f;
     }
     wsb[at] = kb < a.blocks ? ws[kb] : 0.f;
   };
 #pragma unroll
   for (int d = 0; d < D; ++d) fetch_w(warp + d * WARPS, wb[d]);
+  if (a.early) qb_follow();
 #pragma unroll
   for (int d = 0; d < XD; ++d) fetch_x(warp + d * WARPS, d);
   float acc[NT][4];
@@ -130,42 +135,44 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) linear_fp8_tokens_kernel(Lin
     for (int i = 0; i < 4; ++i) part[warp][n * 8 + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[n][i];
   __syncthreads();
   for (int v = threadIdx.x; v < TOK * 16; v += WARPS * 32) {
-    const int tok = v / 16, row = v % 16;
+    const int tok = t0 + v / 16, row = v % 16;
     if (tok >= a.T || n0 + row >= a.N) continue;
-    float s = part[0][tok][row];
+    float s = part[0][v / 16][row];
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) s += part[w][tok][row];
+    for (int w = 1; w < WARPS; ++w) s += part[w][v / 16][row];
     reinterpret_cast<O*>(a.out)[(size_t)tok * a.N + n0 + row] = qb_from_float<O>(s);
   }
 }
 
 template <int NT, int D, int XD, int WARPS, int MINB, typename O>
 void l8f_launch(const LinearFp8Few& a, cudaStream_t stream) {
-  const int grid = (a.N + 15) / 16;
+  const dim3 grid((a.N + 15) / 16, (a.T + NT * 8 - 1) / (NT * 8));
   if (a.K % 32 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 31) == 0) qb_launch(linear_fp8_tokens_kernel<NT, D, XD, WARPS, MINB, true, O>, grid, WARPS * 32, 0, stream, a);
   else qb_launch(linear_fp8_tokens_kernel<NT, D, XD, WARPS, MINB, false, O>, grid, WARPS * 32, 0, stream, a);
 }
 
 }  // namespace
 
-// Whether products of T tokens and a [N, K] matrix are this kernel's: up to 8 tokens all, up to 16 those of at most 32 MB, up to 32 those of a block
-// an SM and 12 MB at most.
-bool qb_linear_fp8_tokens_takes(int T, int K, int N, int sms) {
+// Whether products of T tokens and a [N, K] matrix are this kernel's, by the times above: up to 8 tokens all, up to 16 those of at most 32 MB, up to
+// 32 those of 12 MB, up to 256 those whose bytes times tokens are at most 2^28.
+bool qb_linear_fp8_tokens_takes(int T, int K, int N) {
   const long long bytes = (long long)K * N;
-  return T <= 8 || (T <= 16 && bytes <= 32 << 20) || (T <= 32 && (N + 15) / 16 <= sms && bytes <= 12 << 20);
+  return T <= 8 || (T <= 16 && bytes <= 32 << 20) || (T <= 32 && bytes <= 12 << 20) || (T <= 256 && T * bytes <= 1 << 28);
 }
 
 // K a multiple of 16, x and w on 16 bytes (linear_fp8.cu has looked).  Blocks of four warps where there are two for every SM or
-// more, else of eight, so that few blocks have as many bytes on their way.
-int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int sms,
-                         cudaStream_t stream) {
-  const LinearFp8Few a{(const uint8_t*)x, (const uint8_t*)w, xs, ws, out, T, K, N, (K + FP8_BLOCK - 1) / FP8_BLOCK};
-  const bool many = (N + 15) / 16 >= 2 * sms;
+// more, else of eight, so that few blocks have as many bytes on their way.  More than 16 tokens: tiles of 16, two blocks an SM; of 32, one an SM, where
+// those are one wave and tiles of 16 would be more than a block an SM (32 tokens, 2,048 x 2,048: 3.4 us, with 16 3.7; 4,096 x 1,024: 4.5 and 3.6).
+int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int early,
+                         int sms, cudaStream_t stream) {
+  const LinearFp8Few a{(const uint8_t*)x, (const uint8_t*)w, xs, ws, out, T, K, N, (K + FP8_BLOCK - 1) / FP8_BLOCK, early};
+  const int across = (N + 15) / 16;
+  const bool many = across >= 2 * sms, wide = (long long)across * ((T + 15) / 16) > sms && (long long)across * ((T + 31) / 32) <= sms;
   QB_DISPATCH_DTYPE(out_dtype, O, {
     if (T <= 8 && many) l8f_launch<1, 2, 2, 4, 4, O>(a, stream);
     else if (T <= 8) l8f_launch<1, 2, 2, 8, 2, O>(a, stream);
     else if (T <= 16 && many) l8f_launch<2, 2, 2, 4, 4, O>(a, stream);
-    else if (T <= 16) l8f_launch<2, 2, 2, 8, 2, O>(a, stream);
+    else if (T <= 16 || !wide) l8f_launch<2, 2, 2, 8, 2, O>(a, stream);
     else l8f_launch<4, 2, 2, 8, 1, O>(a, stream);
   });
   QB_LAUNCH_CHECK();

@@ -1382,11 +1382,13 @@ def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> Non
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
-               status: torch.Tensor | None = None) -> None:
+               status: torch.Tensor | None = None, early: bool = False) -> None:
     """``out [T, N] = x [T, K] @ w [N, K].T`` of e4m3 matrices, ``x`` with scales ``[ceil(K / 128), T]`` (``add_rmsnorm_fp8``), ``w`` with a
     scale for every block of 128 x 128, ``[ceil(N / 128), ceil(K / 128)]``.  A block's products are summed by the tensor cores, the blocks
     scaled and summed in float32; ``out`` float32 or bfloat16 (one rounding).  K a multiple of 16; ``x`` and ``w`` on 16 bytes.  The same
-    operands give the same bits in every run.  ``status``: where a bounded wait that ran out is recorded (the outputs are NaN then)."""
+    operands give the same bits in every run.  ``status``: where a bounded wait that ran out is recorded (the outputs are NaN then).
+    ``early``: nothing the two launches before this one do writes ``w`` or ``w_scales`` (the kernels for few tokens start to read them before
+    the launch before has ended)."""
     _want(w, E4M3, "w"); _want(w_scales, torch.float32, "w_scales")
     if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
         raise ValueError("linear_fp8: x, w and out must be matrices")
@@ -1404,8 +1406,8 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         _want(status, torch.int32, "status")
     device, (p_x, p_xs, p_w, p_ws, p_out, p_status) = _addresses(
         "linear_fp8", ("x", "x_scales", "w", "w_scales", "out", "status"), (x, x_scales, w, w_scales, out, status))
-    fn = _entry("qb_linear_fp8", "pppppiiiipp")
-    _check(fn(p_x, p_xs, p_w, p_ws, p_out, _code(out), T, K, N, p_status, _stream_of(device)), "linear_fp8")
+    fn = _entry("qb_linear_fp8", "pppppiiiiipp")
+    _check(fn(p_x, p_xs, p_w, p_ws, p_out, _code(out), T, K, N, int(early), p_status, _stream_of(device)), "linear_fp8")
 
 
 TOKEN_LOGPROBS_MAX_TOP = 64

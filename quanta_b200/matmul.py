@@ -106,11 +106,12 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
 
 def linear_fp8(x: Fp8Rows | torch.Tensor, w: Fp8Weight, out_dtype: torch.dtype, ctx=None) -> torch.Tensor:
     """``x [T, in] @ w [out, in].T`` of 8-bit operands (``x``, if it is a tensor, is brought to 8 bits first); sums are float32, rounded once
-    to ``out_dtype``.  ``ctx``: the step's context, whose status words record a wait in the kernel that ran out."""
+    to ``out_dtype``.  ``ctx``: the step's context, whose status words record a wait in the kernel that ran out; where it says that the weights are
+    settled, a product of few tokens starts to read them before the launch ahead has ended."""
     if not isinstance(x, Fp8Rows):
         x = quantize_rows(x)
     out = torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype, device=x.q.device)
-    kernels.linear_fp8(x.q, x.scales, w.q, w.scales, out, getattr(ctx, "status", None))
+    kernels.linear_fp8(x.q, x.scales, w.q, w.scales, out, getattr(ctx, "status", None), early=getattr(ctx, "settled", False))
     return out
 
 

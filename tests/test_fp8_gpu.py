@@ -320,3 +320,75 @@ def test_empty_calls():
     x, xs, _, _ = _operands(5, 256, 100, 1)
     kernels.linear_fp8(x, xs, w[:0], ws[:0], torch.empty(5, 0, device=DEV))
     torch.cuda.synchronize()
+
+
+# Products of few tokens whose matrix is too large for the kernel without tensor memory: one k block, k that ends inside one, k cut over the blocks
+# of a cluster unevenly, weight rows that end inside a tile, as many tokens as a tile has and one more.
+LARGE_PRODUCTS = [(9, 4112, 9001), (16, 8192, 5000), (17, 4112, 4104), (32, 11008, 4096), (33, 8208, 1003), (48, 2064, 8200), (64, 4240, 1000), (64, 16, 300001),
+                  (50, 65552, 129), (65, 16, 260000), (100, 4112, 1001), (128, 16400, 257), (129, 2064, 2085), (200, 5648, 2000), (257, 16, 5), (257, 144, 200),
+                  (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N", LARGE_PRODUCTS)
+def test_large_product(T, K, N, dtype):
+    from quanta_b200 import kernels
+    ops = _operands(T, K, N, T + K + N)
+    out, again, ahead = (torch.full((T, N), float("nan"), device=DEV, dtype=dtype) for _ in range(3))
+    status = kernels.new_status(DEV)
+    kernels.linear_fp8(*ops, out, status)
+    kernels.linear_fp8(*ops, again, status)
+    kernels.linear_fp8(*ops, ahead, status, early=True)
+    assert int(status[0]) == 0
+    _product_within(out, *ops)
+    assert torch.equal(out, again) and torch.equal(out, ahead)
+
+
+@pytest.mark.parametrize("T", [40, 100])
+def test_nan_stays_in_its_row_and_column_of_a_large_product(T):
+    from quanta_b200 import kernels
+    x, xs, w, ws = _operands(T, 6400, 1100, T)
+    x.view(torch.uint8)[3, 130] = 0x7f
+    w.view(torch.uint8)[77, 9] = 0xff
+    xs[2, 1], ws[2, 1] = float("inf"), float("nan")
+    out = torch.empty(T, 1100, device=DEV)
+    kernels.linear_fp8(x, xs, w, ws, out)
+    want = torch.zeros(T, 1100, dtype=torch.bool, device=DEV)
+    want[[1, 3]], want[:, 77], want[:, 256:384] = True, True, True
+    assert torch.equal(~torch.isfinite(out), want)
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 512, 2048), (7, 4096, 700), (20, 2048, 1024), (40, 512, 512), (20, 8192, 4000), (64, 2048, 4096), (100, 4096, 1024), (300, 512, 640)])
+def test_weights_read_ahead_of_the_rows(T, K, N):
+    """Rows that the launch just before writes, in a chain, eagerly and in a graph: only the weights are read before it has ended."""
+    from quanta_b200 import kernels
+    g = _gen(T)
+    _, _, w, ws = _operands(1, K, N, 3)
+    xs = [_randn(g, T, K) * 4.0 ** i for i in range(6)]
+    q, s = _empty_rows(T, K)
+
+    def chain(outs, early):
+        for x, out in zip(xs, outs):
+            kernels.rows_to_fp8(x, q, s)
+            kernels.linear_fp8(q, s, w, ws, out, early=early)
+
+    want, got, held = (torch.empty(6, T, N, device=DEV) for _ in range(3))
+    for x, out in zip(xs, want):
+        kernels.rows_to_fp8(x, q, s)
+        torch.cuda.synchronize()
+        kernels.linear_fp8(q, s, w, ws, out)
+        torch.cuda.synchronize()
+    chain(got, True)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(held, True)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("T,K,N", [(30, 8192, 4000), (64, 4096, 2100), (100, 4096, 1024)])
+def test_two_large_calls_at_once(T, K, N):
+    test_two_calls_at_once(T, K, N)
