@@ -61,6 +61,9 @@ __device__ __forceinline__ void l8_fma2(float2& c, float ax, float ay, float bx,
       : "+f"(c.x), "+f"(c.y) : "f"(ax), "f"(ay), "f"(bx), "f"(by));
 }
 
+// a map of a tensor on its way before the first copy needs it
+__device__ __forceinline__ void l8_fetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 __device__ __forceinline__ float l8_remote(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -107,7 +110,6 @@ __device__ __forceinline__ void l8_store4(O* row, int n, int N, float4 v) {
 template <int NT, typename O>
 __global__ void __launch_bounds__(L8_FEW_THREADS)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, LinearFp8 a) {
-  if (!a.early) qb_follow();
   constexpr int ADDERS = 4, COLS = NT;
   constexpr uint32_t STAGE = L8_A + NT * L8_BK;
   constexpr int ACC = NT <= 32 ? 8 : 4;
@@ -136,6 +138,8 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     sh.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    l8_fetch_map(&tm_w);
+    l8_fetch_map(&tm_x);
     // the first weights may be asked for before the launch ahead has ended; its tokens are not there yet
     for (int kb = 0; a.early && kb < min(a.stages, k_blocks); ++kb) {
       mbar_expect_tx(smem_u32(&sh.full[kb]), STAGE);
@@ -143,7 +147,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
   }
   // (no tensor memory before it: a block of the launch ahead may still have to get its own)
-  if (a.early) qb_follow();
+  qb_follow();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -345,7 +349,6 @@ template <bool PAIR, typename O>
 __global__ void __launch_bounds__(L8_THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
                   LinearFp8 a, int boxes) {
-  qb_follow();
   constexpr int SIDE = PAIR ? 256 : 128, HALVES = PAIR ? 2 : 1, ACC = 4 / HALVES, COLS = PAIR ? 128 : 64;      // ACC: accumulators a half
   constexpr uint32_t TMEM = 512;
   extern __shared__ unsigned char smem_dyn[];
@@ -376,7 +379,10 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
     sh.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    l8_fetch_map(&tm_w);
+    l8_fetch_map(&tm_x);
   }
+  qb_follow();      // (no tensor memory before it: a block of the launch ahead may still have to get its own)
   if (warp == 1) {
     if constexpr (PAIR) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(TMEM) : "memory");
@@ -706,8 +712,11 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
     const int NT = T <= 16 ? 16 : T <= 32 ? 32 : 64;
     a.t_tiles = 1;
     const long long tiles = (N + L8_M - 1) / L8_M;
+    // Along k as long as the parts are at most one an SM (a k block takes some 0.3 us, joining the parts some 2.5: 32 tokens, 16 tiles, 16 k blocks
+    // 8.4 us uncut, 5.7 in four parts, 5.9 in eight), and once more where a part is still long (86 tiles, 32 k blocks, 64 tokens: 19.7 us, 16.5 in two).
     a.cut = 1;
-    while (a.cut < 8 && tiles * a.cut < sms && a.blocks >= 4 * a.cut) a.cut *= 2;
+    while (a.cut < 8 && tiles * a.cut * 2 <= sms && a.blocks >= (a.cut < 4 ? 8 : 32)) a.cut *= 2;
+    if (a.cut < 8 && tiles * a.cut < sms && a.blocks / a.cut * NT >= 20 * 32) a.cut *= 2;
     a.per = (a.blocks + a.cut - 1) / a.cut;
     const size_t stage = L8_A + (size_t)NT * L8_BK, need = a.cut > 1 ? (size_t)NT * L8_M * 4 : 0;
     int stages = (int)(100 * 1024 / stage);
@@ -737,9 +746,11 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
   a.t_tiles = (T + width - 1) / width;
   const long long tiles = (long long)((N + width - 1) / width) * a.t_tiles;
+  // Along k where that saves more than the joining takes (256 tokens, 4,096 x 4,096, 32 k blocks: 15.3 us uncut, 12.3 in two parts; 16 k blocks and 32 tiles:
+  // 8.1 us, 8.6 in four parts).
   a.cut = 1;
-  if (!pair)
-    while (a.cut < 4 && tiles * a.cut * 2 <= sms && a.blocks >= 4 * a.cut) a.cut *= 2;
+  if (!pair && a.blocks > 16)
+    while (a.cut < 4 && tiles * a.cut * 2 <= sms) a.cut *= 2;
   a.per = (a.blocks + a.cut - 1) / a.cut;
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
   const size_t stage = 2 * L8_A, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;

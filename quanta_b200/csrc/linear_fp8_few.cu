@@ -7,12 +7,12 @@
 // row's bits are the same in every step of as many warps a block.
 //
 // Measured on a B200, one product after another in a graph, weights from memory, microseconds (bytes at 6.5 TB/s / this / tcgen05):
-//   one token    4,096 x 22,016 13.8 / 18.5 / 18.6, 2,048 x 2,048 0.6 / 2.1 / 5.5
-//   8 tokens     2,048 x 11,264 3.5 / 7.2 / 8.7, 5,632 x 2,048 1.8 / 4.5 / 7.5
-//   16           5,632 x 2,048 1.8 / 5.4 / 7.5, 4,096 x 22,016 13.8 / 21.3 / 18.8
-//   32           2,048 x 2,048 0.6 / 3.4 / 6.0, 5,632 x 2,048 1.8 / 7.1 / 8.5, 4,096 x 4,096 2.6 / 10.7 / 8.9, 2,048 x 11,264 3.5 / 13 / 10.4
-//   64           1,024 x 1,024 0.2 / 2.4 / 5.8, 2,048 x 2,048 0.6 / 6.0 / 7.5, 2,048 x 4,096 1.3 / 10.9 / 9.4
-//   96           2,048 x 2,048 0.6 / 8.6 / 7.7;   128: 2,048 x 768 0.2 / 5.1 / 8.0;   256: 1,024 x 1,024 0.2 / 7.3 / 7.6, 2,048 x 768 0.2 / 8.9 / 8.1
+//   one token    4,096 x 22,016 13.8 / 18.5 / 18.5, 512 x 29,000 2.3 / 6.1 / 5.9, 1,024 x 200,000 (4 tokens) 31.3 / 40.8 / 39.9, 16 x 200,000 0.5 / 20.3 / 11.9
+//   8 tokens     4,096 x 4,096 2.6 / 5.5 / 7.8, 2,048 x 2,048 0.6 / 2.1 / 5.1, 1,024 x 1,024 0.2 / 1.7 / 4.4
+//   16           4,096 x 4,096 2.6 / 6.6 / 7.9, 2,048 x 11,264 3.5 / 9.1 / 8.9, 4,096 x 22,016 13.8 / 22.4 / 18.7
+//   32           2,048 x 2,048 0.6 / 3.4 / 5.6, 4,096 x 2,048 1.3 / 5.2 / 7.0, 2,048 x 4,096 1.3 / 6.5 / 5.9, 4,096 x 4,096 2.6 / 10.7 / 8.2
+//   64           1,024 x 1,024 0.2 / 2.4 / 5.7, 2,048 x 2,048 0.6 / 6.4 / 6.6, 2,048 x 4,096 1.3 / 10.8 / 7.0
+//   128          1,024 x 1,024 0.2 / 4.3 / 6.0, 1,024 x 2,048 0.3 / 7.4 / 6.0;   256: 2,048 x 512 0.2 / 6.3 / 8.0;   1,000: 512 x 64 0 / 2.0 / 4.6
 // What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps and a cluster's parts before and behind the bytes; what bounds
 // this one in a large matrix or with many tokens is the issue of instructions (154 a warp for 2 KB and 8 tokens: e4m3 operands of mma.sync are converted
 // to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took the same time; four pieces ahead instead of two a
@@ -153,11 +153,13 @@ void l8f_launch(const LinearFp8Few& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether products of T tokens and a [N, K] matrix are this kernel's, by the times above: up to 8 tokens all, up to 16 those of at most 32 MB, up to
-// 32 those of 12 MB, up to 256 those whose bytes times tokens are at most 2^28.
+// Whether products of T tokens and a [N, K] matrix are this kernel's.  Up to 8 tokens all but those of very many short rows; more as long as its
+// blocks are few for their length, blocks x (K + 4,096) at most 3 x 2^20, by the times above and those of some 200 sizes (K 256 to 11,008, N 512 to 10,000, 9 to 256
+// tokens), of which none is off by more than a tenth.
 bool qb_linear_fp8_tokens_takes(int T, int K, int N) {
-  const long long bytes = (long long)K * N;
-  return T <= 8 || (T <= 16 && bytes <= 32 << 20) || (T <= 32 && bytes <= 12 << 20) || (T <= 256 && T * bytes <= 1 << 28);
+  if (T <= 8) return K >= 1024 || N <= 30000;
+  const long long blocks = (long long)((N + 15) / 16) * ((T + 15) / 16);
+  return blocks * (K + 4096ll) <= 3 << 20;
 }
 
 // K a multiple of 16, x and w on 16 bytes (linear_fp8.cu has looked).  Blocks of four warps where there are two for every SM or

@@ -326,7 +326,8 @@ def test_empty_calls():
 # of a cluster unevenly, weight rows that end inside a tile, as many tokens as a tile has and one more.
 LARGE_PRODUCTS = [(9, 4112, 9001), (16, 8192, 5000), (17, 4112, 4104), (32, 11008, 4096), (33, 8208, 1003), (48, 2064, 8200), (64, 4240, 1000), (64, 16, 300001),
                   (50, 65552, 129), (65, 16, 260000), (100, 4112, 1001), (128, 16400, 257), (129, 2064, 2085), (200, 5648, 2000), (257, 16, 5), (257, 144, 200),
-                  (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500)]
+                  (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500), (33, 8208, 2003), (64, 4240, 2000), (50, 65552, 300), (40, 144, 20001),
+                  (128, 16400, 520), (257, 16, 4100), (300, 2192, 640), (260, 40016, 130), (700, 2320, 384), (1000, 512, 64), (9000, 16, 16), (5, 16, 40001)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -345,20 +346,21 @@ def test_large_product(T, K, N, dtype):
 
 
 @pytest.mark.parametrize("T", [40, 100])
-def test_nan_stays_in_its_row_and_column_of_a_large_product(T):
+@pytest.mark.parametrize("N", [1100, 2100])
+def test_nan_stays_in_its_row_and_column_of_a_large_product(T, N):
     from quanta_b200 import kernels
-    x, xs, w, ws = _operands(T, 6400, 1100, T)
+    x, xs, w, ws = _operands(T, 6400, N, T)
     x.view(torch.uint8)[3, 130] = 0x7f
     w.view(torch.uint8)[77, 9] = 0xff
     xs[2, 1], ws[2, 1] = float("inf"), float("nan")
-    out = torch.empty(T, 1100, device=DEV)
+    out = torch.empty(T, N, device=DEV)
     kernels.linear_fp8(x, xs, w, ws, out)
-    want = torch.zeros(T, 1100, dtype=torch.bool, device=DEV)
+    want = torch.zeros(T, N, dtype=torch.bool, device=DEV)
     want[[1, 3]], want[:, 77], want[:, 256:384] = True, True, True
     assert torch.equal(~torch.isfinite(out), want)
 
 
-@pytest.mark.parametrize("T,K,N", [(1, 512, 2048), (7, 4096, 700), (20, 2048, 1024), (40, 512, 512), (20, 8192, 4000), (64, 2048, 4096), (100, 4096, 1024), (300, 512, 640)])
+@pytest.mark.parametrize("T,K,N", [(1, 512, 2048), (7, 4096, 700), (20, 2048, 1024), (40, 512, 512), (20, 8192, 4000), (64, 2048, 4096), (64, 4096, 2100), (100, 4096, 1024), (300, 512, 640), (300, 2048, 640)])
 def test_weights_read_ahead_of_the_rows(T, K, N):
     """Rows that the launch just before writes, in a chain, eagerly and in a graph: only the weights are read before it has ended."""
     from quanta_b200 import kernels
