@@ -314,16 +314,16 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------
-// More tokens.  A tile is 128 tokens x 128 weight rows, or, for a PAIR of blocks, 256 x 256, of which each block fetches its own 128 tokens and
-// half of the weights and holds the sums of its own tokens.
+// More tokens.  A tile is 128 tokens x 128 weight rows, or, for a PAIR of blocks, 256 tokens x SIDE_N weight rows (256 or 128), of which each block
+// fetches its own 128 tokens and half of the weights and holds the sums of its own tokens.
 //   warp 0     : TMA producer
-//   warps 1, 2 : MMA issuers (of a pair's first block), 4 x tcgen05.mma a job, N = 128.  A pair's k block is two jobs, the weight rows' halves, with
+//   warps 1, 2 : MMA issuers (of a pair's first block), 4 x tcgen05.mma a job, N = 128.  A k block of 256 weight rows is two jobs, the rows' halves, with
 //                accumulators of their own (four in all), so that the addition of one half runs under the products of the other.  An MMA is
 //                taken when the tensor cores are ready for it, and the waits and commits of a k block cost an issuer some 400 cycles besides the
 //                512 of its products, so two take the k blocks in turn.  (One issuer, N = 256, two accumulators: 984 cycles a k block, of which
 //                the tensor cores worked 512.)  The number of stages is even, so that a stage and an accumulator belong to one issuer, which
 //                waits for every phase of their barriers in order.
-//   warps 4-11 : a TMEM lane quadrant and 64 columns (a pair: 128) each: add, then store. They hold up to 128 sums a thread, more registers than
+//   warps 4-11 : a TMEM lane quadrant and half the columns (64 or 128) each: add, then store. They hold up to 128 sums a thread, more registers than
 //                a block of 384 threads can give every one, so the other warps hand some of theirs over; what all have then is at most
 //                what the block was launched with.
 // Pairs walk over the tiles (a block an SM), so that the copies of the next tile run under the stores of the last; a block of a cut product has one.
@@ -331,7 +331,6 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 constexpr int L8_REGS_ADD = 224, L8_REGS_OTHER = 56, L8_REGS_LAUNCH = 168, L8_GROUP = 8;
 static_assert(256 * L8_REGS_ADD + 128 * L8_REGS_OTHER <= L8_THREADS * L8_REGS_LAUNCH, "registers of the launch");
 constexpr int L8_BOX = 32 * 128;            // bytes of a warp's staged part of the output: 32 rows of 128 bytes
-constexpr uint32_t L8_STAGE = 2 * L8_A;     // 128 tokens and 128 weight rows
 struct L8Big {
   uint64_t full[8], empty[8], acc_full[2][4], acc_empty[2][4];      // [half][accumulator]
   uint32_t tmem_base;
@@ -345,11 +344,14 @@ __device__ __forceinline__ void l8_store_box(const CUtensorMap* map, uint32_t fr
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(from) : "memory");
 }
 
-template <bool PAIR, typename O>
+template <bool PAIR, int SIDE_N, typename O>
 __global__ void __launch_bounds__(L8_THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
                   LinearFp8 a, int boxes) {
-  constexpr int SIDE = PAIR ? 256 : 128, HALVES = PAIR ? 2 : 1, ACC = 4 / HALVES, COLS = PAIR ? 128 : 64;      // ACC: accumulators a half
+  static_assert(SIDE_N == 128 || (PAIR && SIDE_N == 256), "a block alone takes 128 weight rows");
+  constexpr int SIDE_T = PAIR ? 256 : 128, HALVES = SIDE_N / 128, ACC = 4 / HALVES, COLS = SIDE_N / 2;      // ACC: accumulators a half
+  constexpr int B_ROWS = PAIR ? SIDE_N / 2 : SIDE_N;      // weight rows that a block fetches
+  constexpr uint32_t STAGE = L8_A + B_ROWS * L8_BK;
   constexpr uint32_t TMEM = 512;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
@@ -357,15 +359,15 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR || a.cut > 1 ? (int)cluster_ctarank() : 0, width = PAIR ? 2 : a.cut;      // blocks of the cluster
   const int k_first = PAIR ? 0 : rank * a.per, k_blocks = max(0, min(a.per, a.blocks - k_first));
-  const int n_tiles = (a.N + SIDE - 1) / SIDE, tiles_all = n_tiles * a.t_tiles;
+  const int n_tiles = (a.N + SIDE_N - 1) / SIDE_N, tiles_all = n_tiles * a.t_tiles;
   const int tile_first = blockIdx.x / width, tile_step = gridDim.x / width;
   volatile int* abort_flag = &sh.abort_flag;
   // a tile's first weight row and this block's first token
   auto place = [&](int tile, int& n0, int& t0) {
     const int per_group = L8_GROUP * n_tiles, group = tile / per_group, in = tile - group * per_group;
     const int high = min(L8_GROUP, a.t_tiles - group * L8_GROUP);
-    n0 = in / high * SIDE;
-    t0 = (group * L8_GROUP + in % high) * SIDE + (PAIR ? rank * 128 : 0);
+    n0 = in / high * SIDE_N;
+    t0 = (group * L8_GROUP + in % high) * SIDE_T + (PAIR ? rank * 128 : 0);
   };
 
   if (threadIdx.x == 0) {
@@ -375,7 +377,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(smem_u32(&sh.acc_full[s / ACC][s % ACC]), 1);
-      mbar_init(smem_u32(&sh.acc_empty[s / ACC][s % ACC]), 8);      // the warps that add it: a half's four of each block of a pair
+      mbar_init(smem_u32(&sh.acc_empty[s / ACC][s % ACC]), (PAIR ? 16 : 8) / HALVES);      // the warps that add it, of each block of a pair
     }
     sh.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -411,14 +413,14 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       for (int tile = tile_first; tile < tiles_all && ok; tile += tile_step) {
         int n0, t0;
         place(tile, n0, t0);
-        if (PAIR) n0 += rank * 128;
+        if (PAIR) n0 += rank * B_ROWS;
 #pragma unroll 1
         for (int kb = 0; kb < k_blocks; ++kb) {
           ok = mbar_wait(smem_u32(&sh.empty[s]), parity, abort_flag);
           if (!ok) break;
-          const uint32_t st = smem_u32(tiles) + (uint32_t)s * L8_STAGE;
+          const uint32_t st = smem_u32(tiles) + (uint32_t)s * STAGE;
           // (a pair: every copy of either block counts on the first block's barrier, which expects both blocks' bytes)
-          if (rank == 0 || !PAIR) mbar_expect_tx(full0 + 8u * s, HALVES * L8_STAGE);
+          if (rank == 0 || !PAIR) mbar_expect_tx(full0 + 8u * s, (PAIR ? 2 : 1) * STAGE);
           if constexpr (PAIR) {
             tma_load_2d_pair(st, &tm_x, kb * L8_BK, t0, bars + 8u * s, pol);
             tma_load_2d_pair(st + L8_A, &tm_w, kb * L8_BK, n0, bars + 8u * s, pol);
@@ -456,7 +458,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 #pragma unroll 1
       for (int turn = (int)first; turn < turns && ok; turn += 2) {
         ok = mbar_wait(smem_u32(&sh.full[s]), full_parity, abort_flag);
-        const uint64_t a_desc = a_first + (uint64_t)(s * (int)(L8_STAGE >> 4)), b_desc = b_first + (uint64_t)(s * (int)(L8_STAGE >> 4));
+        const uint64_t a_desc = a_first + (uint64_t)(s * (int)(STAGE >> 4)), b_desc = b_first + (uint64_t)(s * (int)(STAGE >> 4));
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
           ok = ok && mbar_wait(smem_u32(&sh.acc_empty[h][buf]), empty_parity, abort_flag);
@@ -479,13 +481,13 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
   } else if (warp >= L8_FIRST) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L8_REGS_ADD));
-    constexpr int AHEAD = 4, WS = PAIR ? 2 : 1;
-    const int quad = warp & 3, group = (warp - L8_FIRST) / 4, h = PAIR ? group : 0;
+    constexpr int AHEAD = 4, WS = HALVES;
+    const int quad = warp & 3, group = (warp - L8_FIRST) / 4, h = HALVES == 2 ? group : 0;
     // column i of the warp's sums: weight row n0 + col0 + i / 64 * 128 + i % 64
     const int col0 = group * 64;
-    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(PAIR ? h * ACC * 128 : group * 64);
+    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(HALVES == 2 ? h * ACC * 128 : group * 64);
     const uint32_t full0 = smem_u32(&sh.acc_full[h][0]), empty0 = PAIR ? mapa_u32(smem_u32(&sh.acc_empty[h][0]), 0u) : smem_u32(&sh.acc_empty[h][0]);
-    const uint32_t staged = smem_u32(tiles) + (uint32_t)a.stages * L8_STAGE + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
+    const uint32_t staged = smem_u32(tiles) + (uint32_t)a.stages * STAGE + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
     float x_ahead[AHEAD], w_ahead[WS][AHEAD];
     const float *xs = a.xs, *ws = a.ws;
     bool has_x = false, has_w[WS];
@@ -507,7 +509,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       }
     };
     scales_of(tile_first);
-    uint32_t turn = 0u;
+    uint32_t turn = 0u, at_box = 0u;
     bool ok = true;
 #pragma unroll 1
     for (int tile = tile_first; tile < tiles_all; tile += tile_step) {
@@ -579,7 +581,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         for (int b = 0; b < COLS / PER; ++b) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the copy out of this box, two ago
           __syncwarp();
-          const uint32_t box = staged + (uint32_t)(b & 1) * L8_BOX, to = box + (uint32_t)lane * 128;
+          const uint32_t box = staged + at_box, to = box + (uint32_t)lane * 128;
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             uint32_t w[4];
@@ -603,6 +605,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             if (t0 + quad * 32 < a.T && n < a.N) l8_store_box(&tm_out, box, n, t0 + quad * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
+          at_box ^= (uint32_t)L8_BOX;
         }
       } else if (t0 + row < a.T) {
         O* dst = out + (size_t)(t0 + row) * a.N;
@@ -672,10 +675,10 @@ int l8_few(CUtensorMap& tm_w, CUtensorMap& tm_x, LinearFp8& a, unsigned grid, si
   void* args[] = {&tm_w, &tm_x, &a};
   return l8_cluster_launch((const void*)linear_fp8_few_kernel<NT, O>, args, grid, L8_FEW_THREADS, (unsigned)a.cut, smem, stream);
 }
-template <bool PAIR, typename O>
+template <bool PAIR, int SIDE_N, typename O>
 int l8_many(CUtensorMap& tm_w, CUtensorMap& tm_x, CUtensorMap& tm_out, LinearFp8& a, int boxes, unsigned grid, size_t smem, cudaStream_t stream) {
   // the registers that the block's warps share out are those of the launch
-  const void* kern = (const void*)linear_fp8_kernel<PAIR, O>;
+  const void* kern = (const void*)linear_fp8_kernel<PAIR, SIDE_N, O>;
   cudaFuncAttributes attr;
   const cudaError_t err = cudaFuncGetAttributes(&attr, kern);
   if (err != cudaSuccess) return (int)err;
@@ -738,34 +741,39 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
     return 0;
   }
   // Pairs of blocks where tiles of 128 x 128 would be more than one for every SM (768 tokens, 4,096 x 4,096: 20 us, 29 with single blocks; 512, one tile an
-  // SM: 20 and 15), but for tokens that fill half a pair's tile at most; else single blocks, cut along k where they are few.
-  const long long singles = (long long)((T + 127) / 128) * ((N + 127) / 128);
-  const bool pair = T > 128 && singles > sms;
-  const int width = pair ? 256 : 128;
-  const size_t size = out_dtype == QB_F32 ? 4 : 2;
-  const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
-  a.t_tiles = (T + width - 1) / width;
-  const long long tiles = (long long)((N + width - 1) / width) * a.t_tiles;
+  // SM: 19 and 15), but for tokens that fill half a pair's tile at most.  256 weight rows a pair or 128, whichever makes the shorter waves: a tile of
+  // 128 takes some 0.65 of one of 256 (256 tokens, 4,096 x 22,016: 38 us in two waves of the one, 34.5 in three of the other; 1,024: 89 and 109).
+  // Else single blocks, cut along k where they are few, or, where they are not cut and k is long, pairs with 128 rows, which fetch three quarters
+  // of the bytes (512 tokens, 11,008 x 4,096: 35 and 30 us).
+  const long long singles = (long long)((T + 127) / 128) * ((N + 127) / 128), t_pairs = (T + 255) / 256;
+  const long long waves_256 = (t_pairs * ((N + 255) / 256) * 2 + sms - 1) / sms, waves_128 = (t_pairs * ((N + 127) / 128) * 2 + sms - 1) / sms;
   // Along k where that saves more than the joining takes (256 tokens, 4,096 x 4,096, 32 k blocks: 15.3 us uncut, 12.3 in two parts; 16 k blocks and 32 tiles:
   // 8.1 us, 8.6 in four parts).
   a.cut = 1;
-  if (!pair && a.blocks > 16)
-    while (a.cut < 4 && tiles * a.cut * 2 <= sms) a.cut *= 2;
+  if (a.blocks > 16)
+    while (a.cut < 4 && singles * a.cut * 2 <= sms) a.cut *= 2;
+  const bool pair = T > 128 && (singles > sms || (a.cut == 1 && a.blocks >= 32));
+  const int side = pair && singles > sms && waves_256 * 20 <= waves_128 * 13 ? 256 : 128, w_rows = pair && side == 128 ? 64 : 128;      // weight rows of a block's stage
+  const size_t size = out_dtype == QB_F32 ? 4 : 2;
+  const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
+  a.t_tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128);
+  const long long tiles = (long long)((N + side - 1) / side) * a.t_tiles;
   a.per = (a.blocks + a.cut - 1) / a.cut;
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
-  const size_t stage = 2 * L8_A, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;
-  a.stages = a.cut > 1 ? 6 : 4;
+  const size_t stage = L8_A + (size_t)w_rows * L8_BK, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;
+  a.stages = a.cut > 1 || w_rows == 64 ? 6 : 4;
   const size_t smem = stage * a.stages + staged + 1024;
-  rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, 128, bytes);
+  rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, (uint32_t)w_rows, bytes);
   if (!rc) rc = l8_map(&tm_x, x, (uint64_t)T, (uint64_t)K, 1, 128, bytes);
   if (!rc && boxes)
     rc = l8_map(&tm_out, out, (uint64_t)T, (uint64_t)N, (uint32_t)size, 32, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
   if (rc) return rc;
   if (!boxes) tm_out = tm_x;      // not used
-  const unsigned grid = pair ? (unsigned)(sms / 2 * 2) : (unsigned)(tiles * a.cut);
+  const unsigned grid = pair ? (unsigned)(tiles * 2 < sms / 2 * 2 ? tiles * 2 : sms / 2 * 2) : (unsigned)(tiles * a.cut);
   QB_DISPATCH_DTYPE(out_dtype, O, {
-    if (pair) rc = l8_many<true, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
-    else rc = l8_many<false, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
+    if (pair && side == 256) rc = l8_many<true, 256, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
+    else if (pair) rc = l8_many<true, 128, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
+    else rc = l8_many<false, 128, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
   });
   if (rc) return rc;
   QB_LAUNCH_CHECK();

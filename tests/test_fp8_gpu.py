@@ -327,7 +327,8 @@ def test_empty_calls():
 LARGE_PRODUCTS = [(9, 4112, 9001), (16, 8192, 5000), (17, 4112, 4104), (32, 11008, 4096), (33, 8208, 1003), (48, 2064, 8200), (64, 4240, 1000), (64, 16, 300001),
                   (50, 65552, 129), (65, 16, 260000), (100, 4112, 1001), (128, 16400, 257), (129, 2064, 2085), (200, 5648, 2000), (257, 16, 5), (257, 144, 200),
                   (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500), (33, 8208, 2003), (64, 4240, 2000), (50, 65552, 300), (40, 144, 20001),
-                  (128, 16400, 520), (257, 16, 4100), (300, 2192, 640), (260, 40016, 130), (700, 2320, 384), (1000, 512, 64), (9000, 16, 16), (5, 16, 40001)]
+                  (128, 16400, 520), (257, 16, 4100), (300, 2192, 640), (260, 40016, 130), (700, 2320, 384), (1000, 512, 64), (9000, 16, 16), (5, 16, 40001),
+                  (400, 4112, 3000), (512, 5648, 4001), (1030, 4240, 2000), (1300, 4096, 4096), (200, 2064, 20008), (200, 2064, 20001)]      # pairs with 128 weight rows
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
