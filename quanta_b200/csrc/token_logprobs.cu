@@ -15,8 +15,8 @@
 //
 // A row is cut over the blocks of a cluster where rows are few; the first block joins what the others leave in shared memory.
 // Bound by the row's bytes; in bfloat16 by the issue of instructions (two additions, a product, two exponentials and a multiply-add for two numbers);
-// for a few rows by the chain of a read, the joins and the second read.  Measured on a B200, with 20 tokens a row: 2,048 rows of 200,064 float32 270 us (6.1
-// TB/s), bfloat16 178 us (4.6 TB/s); 64 rows of 32,000 10.2 us, one row of 200,064 9.8 us.
+// for a few rows by the chain of a read, the joins and the second read.  Measured on a B200, with 20 tokens a row: 2,048 rows of 200,064 float32 257 us (6.4
+// TB/s), bfloat16 162 us (5.1 TB/s); 64 rows of 32,000 9.9 us, one row of 200,064 9.2 us.
 #include "common.cuh"
 
 namespace {
@@ -252,8 +252,8 @@ __device__ __forceinline__ uint32_t tl_of_first(const void* p) {
   return at;
 }
 
-// AHEAD: pieces a thread has on their way while it works on as many
-template <typename T, int THREADS, int AHEAD>
+// AHEAD: pieces a thread has on their way while it works on as many.  LONG: rows whose parts have more than TL_SLOTS times 512 bytes
+template <typename T, int THREADS, int AHEAD, bool LONG>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(TokenLogprobs a) {
   qb_follow();
   __shared__ TlShared sh;
@@ -274,10 +274,12 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(TokenLogprobs a
   float my_top = -INFINITY;      // NaN aside
   float2 s2 = make_float2(0.f, 0.f), u2 = s2;
   uint4 q[AHEAD], q_next[AHEAD];
-  // slot (b >> shift) * WARPS + warp: the pieces of the warp's turns (b >> shift) << shift and on, a turn being 32 pieces
+  // slot (b >> shift) * WARPS + warp: the pieces of the warp's turns (b >> shift) << shift and on, a turn being 32 pieces.  (The shift of every row's
+  // slots, long or not, took 8% of the time in float32, 12% in bfloat16, which are bound by the issue of instructions as much as by memory.)
   const int turns = (p_hi - p_lo + THREADS - 1) / THREADS;
   int shift = 0, turn = 0;
-  while (((turns - 1) >> shift) * WARPS + WARPS > TL_SLOTS) ++shift;
+  if (LONG)
+    while (((turns - 1) >> shift) * WARPS + WARPS > TL_SLOTS) ++shift;
   {
     for (int k = lane; k <= (turns - 1) >> shift; k += 32) sh.slots[k * WARPS + warp] = -INFINITY;
     __syncwarp();
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(TokenLogprobs a
       top = fmaxf(top, of_piece);
       if (lane == 0) {      // (turns behind the last have slots that nobody looks at)
         float* slot = &sh.slots[((turn + j) >> shift) * WARPS + warp];
-        *slot = shift == 0 ? of_turn : tl_max_nan(*slot, of_turn);
+        *slot = !LONG ? of_turn : tl_max_nan(*slot, of_turn);
       }
     }
     if (top > my_top) {
@@ -530,7 +532,11 @@ extern "C" int qb_token_logprobs(const void* logits, int dtype, long long stride
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   QB_DISPATCH_DTYPE(dtype, T, {
-    auto kern = threads == 512 ? token_logprobs_kernel<T, 512, 4> : token_logprobs_kernel<T, 256, 4>;
+    // (a block's slots: its pieces, a turn of its threads at a time)
+    const long long share = ((long long)V / (16 / (int)sizeof(T)) + 2 + a.cut - 1) / a.cut;
+    const bool is_long = (share + threads - 1) / threads * (threads / 32) > TL_SLOTS;
+    auto kern = threads == 512 ? (is_long ? token_logprobs_kernel<T, 512, 4, true> : token_logprobs_kernel<T, 512, 4, false>)
+                               : (is_long ? token_logprobs_kernel<T, 256, 4, true> : token_logprobs_kernel<T, 256, 4, false>);
     if (a.cut > 8) err = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kern, a);
   });
