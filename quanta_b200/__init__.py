@@ -1,7 +1,7 @@
 """quanta_b200: a small, whole inference engine for one B200 (sm_100a), one model architecture at a
 time, from a model folder (config.json + safetensors) to tokens.
 
-Public entry points: ``generate`` (programmatic), ``python -m quanta_b200 generate`` (command line),
+Public entry points: ``generate`` (programmatic), ``python -m quanta_b200 generate`` and ``score`` (command line),
 ``bin/trace_run`` (replay of given token ids, logits out).
 """
 

@@ -16,7 +16,7 @@
 // A row is cut over the blocks of a cluster where rows are few; the first block joins what the others leave in shared memory.
 // Bound by the row's bytes; in bfloat16 by the issue of instructions (two additions, a product, two exponentials and a multiply-add for two numbers);
 // for a few rows by the chain of a read, the joins and the second read.  Measured on a B200, with 20 tokens a row: 2,048 rows of 200,064 float32 257 us (6.4
-// TB/s), bfloat16 162 us (5.1 TB/s); 64 rows of 32,000 9.9 us, one row of 200,064 9.2 us.
+// TB/s), bfloat16 162 us (5.1 TB/s); 64 bfloat16 rows of 32,000 (5 tokens) 10 us, one row of 200,064 9.5 us.
 #include "common.cuh"
 
 namespace {
