@@ -395,3 +395,83 @@ def test_weights_read_ahead_of_the_rows(T, K, N):
 @pytest.mark.parametrize("T,K,N", [(30, 8192, 4000), (64, 4096, 2100), (100, 4096, 1024)])
 def test_two_large_calls_at_once(T, K, N):
     test_two_calls_at_once(T, K, N)
+
+
+@pytest.mark.parametrize("T,N", [(140000, 16400), (140000, 16401)])
+def test_product_of_more_than_32_bits_of_numbers(T, N):
+    from quanta_b200 import kernels
+    K = 128
+    g = _gen(T)
+    _, _, w, ws = _operands(1, K, N, 1)
+    some, scale = _operands(1000, K, 8, 2)[:2]
+    pick = torch.randint(0, 1000, (T,), device=DEV, generator=g)
+    x, xs = some.view(torch.uint8)[pick].view(E4M3), scale[:, pick].contiguous()
+    out = torch.empty(T, N, device=DEV, dtype=torch.bfloat16)
+    kernels.linear_fp8(x, xs, w, ws, out)
+    few = torch.empty(1000, N, device=DEV, dtype=torch.bfloat16)
+    kernels.linear_fp8(some, scale, w, ws, few)
+    _product_within(few, some, scale, w, ws)
+    for t0 in (0, 65536, 130900, T - 1000):
+        assert torch.equal(out[t0: t0 + 1000], few[pick[t0: t0 + 1000]])
+
+
+def test_rows_of_more_than_32_bits_of_numbers():
+    from quanta_b200 import kernels
+    g = _gen(9)
+    n, width = 100000, 11008
+    some = (2 * _randn(g, 500, 2 * width)).bfloat16()
+    pick = torch.randint(0, 500, (n,), device=DEV, generator=g)
+    q, s = _empty_rows(n, width)
+    kernels.glu_act_fp8(some[pick], q, s)
+    q0, s0 = _empty_rows(500, width)
+    kernels.glu_act_fp8(some, q0, s0)
+    ends = torch.cat([torch.arange(1000), torch.arange(n - 1000, n)]).to(DEV)
+    assert torch.equal(q.view(torch.uint8)[ends], q0.view(torch.uint8)[pick[ends]]) and torch.equal(s[:, ends], s0[:, pick[ends]])
+    n, H = 540000, 4096
+    some, w = _randn(g, 500, H), 1 + 0.1 * _randn(g, H)
+    pick = torch.randint(0, 500, (n,), device=DEV, generator=g)
+    q, s = _empty_rows(n, H)
+    kernels.add_rmsnorm_fp8(some[pick], None, w, 1e-5, q, s)
+    q0, s0 = _empty_rows(500, H)
+    kernels.add_rmsnorm_fp8(some, None, w, 1e-5, q0, s0)
+    ends = torch.cat([torch.arange(1000), torch.arange(n - 1000, n)]).to(DEV)
+    assert torch.equal(q.view(torch.uint8)[ends], q0.view(torch.uint8)[pick[ends]]) and torch.equal(s[:, ends], s0[:, pick[ends]])
+
+
+def test_first_call_inside_a_capture():
+    """Nothing that a kernel needs at its first launch keeps it from being captured: each in a process of its own kind of call."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from quanta_b200 import kernels, fp8
+dev = "cuda:0"
+kernels.lib().unit("fp8"); kernels.lib().unit("scores")
+cases = [(1, 512, 640), (24, 512, 640), (30, 4224, 8000), (60, 4224, 8000), (100, 4224, 1000), (300, 2176, 640), (600, 4224, 4000), (2000, 512, 4000)]
+held = []
+x = [torch.randn(T, K, device=dev) for T, K, N in cases]
+w = [fp8.quantize_weight(torch.randn(N, K, device=dev)) for T, K, N in cases]
+logits = [torch.randn(n, 50000, device=dev) for n in (1, 200)]
+torch.cuda.synchronize()
+def run():
+    outs = []
+    for a, b in zip(x, w):
+        r = fp8.quantize_rows(a)
+        out = torch.empty(a.shape[0], b.shape[0], device=dev)
+        kernels.linear_fp8(r.q, r.scales, b.q, b.scales, out)
+        outs.append(out)
+    for l in logits:
+        en, ids, best = torch.empty(l.shape[0], device=dev), torch.empty(l.shape[0], 5, device=dev, dtype=torch.int32), torch.empty(l.shape[0], 5, device=dev)
+        kernels.token_logprobs(l, None, None, en, ids, best)
+        outs += [en, ids, best]
+    return outs
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, run()))
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]

@@ -231,3 +231,18 @@ def test_rows_of_the_lowest_numbers(n, dtype):
         assert torch.all(((got.double() - want).abs() <= tol[:, None] * (8 + log_s[:, None]) + 4 * U * want.abs())[fine])
     ent = torch.special.entr(torch.softmax(d, 1)).sum(1)
     assert torch.all((en[keep].double() - ent).abs() <= tol * 16 * (1 + ent))
+
+
+def test_more_than_32_bits_of_numbers():
+    g = _gen(8)
+    n, V = 11000, 200064
+    some = torch.randn(50, V, device=DEV, generator=g).bfloat16()
+    pick = torch.randint(0, 50, (n,), device=DEV, generator=g)
+    t = torch.randint(0, V, (50,), device=DEV, generator=g).to(torch.int32)
+    want = _scores(some, t, 7)
+    got = _scores(some[pick], t[pick].contiguous(), 7)
+    # few rows are cut over several blocks, so the sums differ: by twice 2^-21 + (V / 512 + 100) u = 3e-5, the entropy by that times 1 + 2 a, a < 8
+    assert torch.equal(got[2], want[2][pick])
+    for k, tol in ((0, 6e-5), (1, 6e-5 * 17), (3, 6e-5)):
+        assert torch.all((got[k] - want[k][pick]).abs() <= tol + 8 * U * want[k][pick].abs())
+    _check(some, t, 7)
