@@ -1287,26 +1287,31 @@ def _addresses(what: str, names: tuple, tensors: tuple, strided: int = -1) -> tu
     device = tensors[0].get_device()
     if device < 0 or device != _current_device():
         raise ValueError(f"{what}: {names[0]} is on {tensors[0].device}, which is not the current CUDA device")
-    for i, t in enumerate(tensors):
-        if t is not None and (t.get_device() != device or not (t.is_contiguous() or i == strided)):
-            raise ValueError(f"{what}: {names[i]} must be contiguous and on {tensors[0].device}, it is on {t.device}")
-    return device, [None if t is None else t.data_ptr() for t in tensors]
+    at = []
+    for t in tensors:
+        if t is None:
+            at.append(None)
+        elif t.get_device() == device and (t.is_contiguous() or len(at) == strided):
+            at.append(t.data_ptr())
+        else:
+            raise ValueError(f"{what}: {names[len(at)]} must be contiguous and on {tensors[0].device}, it is on {t.device}")
+    return device, at
 
 
 def _stream_of(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _sizes(what: str, *sizes: int) -> None:
-    if max(sizes) > MOST_ROWS:
-        raise ValueError(f"{what}: sizes of at most {MOST_ROWS} are taken, got {max(sizes)}")
+def _sizes(what: str, a: int, b: int = 0) -> None:
+    if a > MOST_ROWS or b > MOST_ROWS:
+        raise ValueError(f"{what}: sizes of at most {MOST_ROWS} are taken, got {max(a, b)}")
 
 
 def _fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, cols: int, name: str) -> None:
-    _want(q, E4M3, name); _want(scales, torch.float32, f"the scales of {name}")
+    _want(q, E4M3, name); _want(scales, torch.float32, "the scales of a matrix of 8 bits")
     blocks = -(-cols // FP8_BLOCK)
     _sizes(what, n, cols)
-    if tuple(q.shape) != (n, cols) or tuple(scales.shape) != (blocks, n):
+    if q.shape != (n, cols) or scales.shape != (blocks, n):      # (torch.Size is a tuple)
         raise ValueError(f"{what}: {name} must be [{n}, {cols}] and its scales [{blocks}, {n}], got {tuple(q.shape)} and {tuple(scales.shape)}")
 
 
@@ -1324,8 +1329,9 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: torch.Tensor | None, weight: torch.T
     T, H = h.shape
     S = 1
     if delta is not None:
-        S = delta.shape[1] if delta.dim() == 3 else 1
-        if delta.dim() not in (2, 3) or delta.shape[0] != T or delta.shape[-1] != H or S < 1:
+        shape = delta.shape
+        S = shape[1] if len(shape) == 3 else 1
+        if len(shape) not in (2, 3) or shape[0] != T or shape[-1] != H or S < 1:
             raise ValueError("add_rmsnorm_fp8: delta shape mismatch")
     if delta_gain is not None:
         _want(delta_gain, torch.float32, "delta_gain")
@@ -1351,9 +1357,10 @@ def glu_act_fp8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, 
                 limit: float = 0.0, alpha: float = 1.0) -> None:
     """``glu_act`` whose result comes out in e4m3 with scales as those of ``add_rmsnorm_fp8``: ``gate_up`` ``[n, 2 I]`` float32 or bfloat16,
     ``out`` ``[n, I]``, ``scales`` ``[ceil(I / 128), n]``.  Nothing is rounded between the activation and e4m3."""
-    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+    shape = gate_up.shape
+    if len(shape) != 2 or shape[1] % 2:
         raise ValueError("glu_act_fp8: gate_up must be [n, 2 I]")
-    n, two_i = gate_up.shape
+    n, two_i = shape
     if bias is not None:
         _want(bias, torch.float32, "bias")
         if bias.numel() != two_i:
@@ -1363,13 +1370,13 @@ def glu_act_fp8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, 
     if kind == GLU_CLAMPED and not limit > 0:
         raise ValueError("glu_act_fp8: the clamped form needs a positive limit")
     _fp8_rows("glu_act_fp8", out, scales, n, two_i // 2, "out")
-    _act_fp8("glu_act_fp8", gate_up, bias, out, scales, two_i // 2, kind, limit, alpha)
+    _act_fp8("glu_act_fp8", gate_up, bias, out, scales, n, two_i // 2, kind, limit, alpha)
 
 
-def _act_fp8(what: str, x, bias, out, scales, cols: int, kind: int, limit: float, alpha: float) -> None:
+def _act_fp8(what: str, x, bias, out, scales, n: int, cols: int, kind: int, limit: float, alpha: float) -> None:
     device, (p_x, p_bias, p_out, p_scales) = _addresses(what, ("the input", "bias", "out", "scales"), (x, bias, out, scales))
     fn = _entry("qb_act_fp8", "pipppiiiffp")
-    _check(fn(p_x, _code(x), p_bias, p_out, p_scales, x.shape[0], cols, int(kind), limit, alpha, _stream_of(device)), what)
+    _check(fn(p_x, _code(x), p_bias, p_out, p_scales, n, cols, int(kind), limit, alpha, _stream_of(device)), what)
 
 
 def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1378,7 +1385,7 @@ def rows_to_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> Non
         raise ValueError("rows_to_fp8: x must be [n, K]")
     n, K = x.shape
     _fp8_rows("rows_to_fp8", out, scales, n, K, "out")
-    _act_fp8("rows_to_fp8", x, None, out, scales, K, 3, 0.0, 1.0)
+    _act_fp8("rows_to_fp8", x, None, out, scales, n, K, 3, 0.0, 1.0)
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
@@ -1393,12 +1400,12 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
         raise ValueError("linear_fp8: x, w and out must be matrices")
     T, K = x.shape
-    N = w.shape[0]
+    N, w_cols = w.shape
     _sizes("linear_fp8", N)
     _fp8_rows("linear_fp8", x, x_scales, T, K, "x")
-    if w.shape[1] != K or tuple(out.shape) != (T, N):
+    if w_cols != K or out.shape != (T, N):
         raise ValueError(f"linear_fp8: w {tuple(w.shape)} and out {tuple(out.shape)} do not fit x {tuple(x.shape)}")
-    if tuple(w_scales.shape) != (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK)):
+    if w_scales.shape != (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK)):
         raise ValueError(f"linear_fp8: w_scales must be [{-(-N // FP8_BLOCK)}, {-(-K // FP8_BLOCK)}], got {tuple(w_scales.shape)}")
     if K == 0 or K % 16:
         raise ValueError(f"linear_fp8: K must be a positive multiple of 16, got {K}")
@@ -1421,9 +1428,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
     is None is not wanted.  A logit of -inf is a token of probability zero.  A row with a NaN or +inf, or with nothing but -inf, has NaN for
     all numbers, and its tokens in the order of the logits with NaN as -inf.  A token outside the vocabulary is recorded in ``status``; its
     log probability is NaN."""
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-        raise ValueError("token_logprobs: logits must be [n, V] with rows of neighbouring numbers")
-    n, V = logits.shape
+    if logits.dim() != 2:
+        raise ValueError("token_logprobs: logits must be [n, V]")
+    (n, V), (stride, step) = logits.shape, logits.stride()
+    if (V > 1 and step != 1) or (n > 1 and stride < V):
+        raise ValueError("token_logprobs: logits must be rows of neighbouring numbers")
     if V == 0:
         raise ValueError("token_logprobs: an empty vocabulary")
     _sizes("token_logprobs", n, V)
@@ -1434,13 +1443,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
     for t, name, dtype in ((tokens, "tokens", torch.int32), (logprob, "logprob", torch.float32), (entropy, "entropy", torch.float32)):
         if t is not None:
             _want(t, dtype, name)
-            if tuple(t.shape) != (n,):
+            if t.shape != (n,):
                 raise ValueError(f"token_logprobs: {name} must be [{n}], got {tuple(t.shape)}")
     top = 0
     if ids is not None:
         _want(ids, torch.int32, "ids"); _want(best, torch.float32, "best")
-        top = ids.shape[1] if ids.dim() == 2 else -1
-        if top < 0 or tuple(ids.shape) != (n, top) or ids.shape != best.shape:
+        shape = ids.shape
+        top = shape[1] if len(shape) == 2 else -1
+        if top < 0 or shape[0] != n or shape != best.shape:
             raise ValueError("token_logprobs: ids and best must be [n, k]")
         if top > min(V, TOKEN_LOGPROBS_MAX_TOP):
             raise ValueError(f"token_logprobs: {top} tokens a row of {V}; at most {TOKEN_LOGPROBS_MAX_TOP} are taken, and no more than there are")
@@ -1450,7 +1460,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
         "token_logprobs", ("logits", "tokens", "logprob", "entropy", "ids", "best", "status"),
         (logits, tokens, logprob, entropy, ids if top else None, best if top else None, status), strided=0)
     fn = _entry("qb_token_logprobs", "pilpppppiiipp")
-    _check(fn(p_x, _code(logits), logits.stride(0), p_t, p_lp, p_en, p_ids, p_best, n, V, top, p_status, _stream_of(device)), "token_logprobs")
+    _check(fn(p_x, _code(logits), stride, p_t, p_lp, p_en, p_ids, p_best, n, V, top, p_status, _stream_of(device)), "token_logprobs")
 
 
 def split2_bf16(x) -> torch.Tensor:
