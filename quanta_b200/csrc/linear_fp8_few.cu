@@ -16,7 +16,7 @@
 // What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps and a cluster's parts before and behind the bytes; what bounds
 // this one in a large matrix or with many tokens is the issue of instructions (154 a warp for 2 KB and 8 tokens: e4m3 operands of mma.sync are converted
 // to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took the same time; four pieces ahead instead of two a
-// longer one (fewer warps).  Weights asked for before the launch ahead has ended (`early`): norm, product, activation and product of 4,096 x 11,008 for
+// longer one in blocks of four warps (fewer of them).  Weights asked for before the launch ahead has ended (`early`): norm, product, activation and product of 4,096 x 11,008 for
 // one token 33.0 -> 32.2 us, for 32 38.1 -> 35.8, of 2,048 x 5,632 15.0 -> 13.7 and 22.5 -> 21.1.
 #include "fp8.cuh"
 
@@ -163,7 +163,9 @@ bool qb_linear_fp8_tokens_takes(int T, int K, int N) {
 }
 
 // K a multiple of 16, x and w on 16 bytes (linear_fp8.cu has looked).  Blocks of four warps where there are two for every SM or
-// more, else of eight, so that few blocks have as many bytes on their way.  More than 16 tokens: tiles of 16, two blocks an SM; of 32, one an SM, where
+// more, else of eight, so that few blocks have as many bytes on their way, and three pieces ahead
+// (one token, 5,632 x 2,048 4.3 -> 3.8 us, 16,384 x 2,048 12.0 -> 10.5).  Four blocks an SM, or five, with less ahead, where that is one wave instead of two (4,096 x
+// 11,008 12.3 -> 10.9 us; 4,096 x 14,336 13.6 and 15.8, 4,096 x 22,016 18.7 and 19.0).  More than 16 tokens: tiles of 16, two blocks an SM; of 32, one an SM, where
 // those are one wave and tiles of 16 would be more than a block an SM (32 tokens, 2,048 x 2,048: 3.4 us, with 16 3.7; 4,096 x 1,024: 4.5 and 3.6).
 int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int early,
                          int sms, cudaStream_t stream) {
@@ -171,8 +173,9 @@ int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const fl
   const int across = (N + 15) / 16;
   const bool many = across >= 2 * sms, wide = (long long)across * ((T + 15) / 16) > sms && (long long)across * ((T + 31) / 32) <= sms;
   QB_DISPATCH_DTYPE(out_dtype, O, {
-    if (T <= 8 && many) l8f_launch<1, 2, 2, 4, 4, O>(a, stream);
-    else if (T <= 8) l8f_launch<1, 2, 2, 8, 2, O>(a, stream);
+    if (T <= 8 && many && across > 4 * sms && across <= 5 * sms) l8f_launch<1, 2, 1, 4, 5, O>(a, stream);
+    else if (T <= 8 && many) l8f_launch<1, 2, 2, 4, 4, O>(a, stream);
+    else if (T <= 8) l8f_launch<1, 3, 3, 8, 2, O>(a, stream);
     else if (T <= 16 && many) l8f_launch<2, 2, 2, 4, 4, O>(a, stream);
     else if (T <= 16 || !wide) l8f_launch<2, 2, 2, 8, 2, O>(a, stream);
     else l8f_launch<4, 2, 2, 8, 1, O>(a, stream);
