@@ -314,7 +314,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------
-// More tokens.  A tile is 128 tokens x 128 weight rows, or, for a PAIR of blocks, 256 tokens x SIDE_N weight rows (256 or 128), of which each block
+// More tokens.  A tile is 128 tokens x SIDE_N weight rows (128 or 256), or, for a PAIR of blocks, 256 tokens x SIDE_N weight rows (256 or 128), of which each block
 // fetches its own 128 tokens and half of the weights and holds the sums of its own tokens.
 //   warp 0     : TMA producer
 //   warps 1, 2 : MMA issuers (of a pair's first block), 4 x tcgen05.mma a job, N = 128.  A k block of 256 weight rows is two jobs, the rows' halves, with
@@ -348,8 +348,9 @@ template <bool PAIR, int SIDE_N, typename O>
 __global__ void __launch_bounds__(L8_THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
                   LinearFp8 a, int boxes) {
-  static_assert(SIDE_N == 128 || (PAIR && SIDE_N == 256), "a block alone takes 128 weight rows");
-  constexpr int SIDE_T = PAIR ? 256 : 128, HALVES = SIDE_N / 128, ACC = 4 / HALVES, COLS = SIDE_N / 2;      // ACC: accumulators a half
+  static_assert(SIDE_N == 128 || SIDE_N == 256, "weight rows of a tile");
+  constexpr int SIDE_T = PAIR ? 256 : 128, HALVES = PAIR ? SIDE_N / 128 : 1, MMA_N = PAIR ? 128 : SIDE_N, COLS = SIDE_N / 2;
+  constexpr int ACC = SIDE_N == 128 ? 4 : 2;      // accumulators a half
   constexpr int B_ROWS = PAIR ? SIDE_N / 2 : SIDE_N;      // weight rows that a block fetches
   constexpr uint32_t STAGE = L8_A + B_ROWS * L8_BK;
   constexpr uint32_t TMEM = 512;
@@ -375,7 +376,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       mbar_init(smem_u32(&sh.full[s]), 1);
       mbar_init(smem_u32(&sh.empty[s]), 1);
     }
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < HALVES * ACC; ++s) {
       mbar_init(smem_u32(&sh.acc_full[s / ACC][s % ACC]), 1);
       mbar_init(smem_u32(&sh.acc_empty[s / ACC][s % ACC]), (PAIR ? 16 : 8) / HALVES);      // the warps that add it, of each block of a pair
     }
@@ -447,7 +448,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
   } else if (warp < 3) {
     if (lane == 0 && (rank == 0 || !PAIR)) {
-      const uint32_t idesc = umma_idesc_e4m3(PAIR ? 256 : 128, 128), first = (uint32_t)warp - 1u;
+      const uint32_t idesc = umma_idesc_e4m3(PAIR ? 256 : 128, MMA_N), first = (uint32_t)warp - 1u;
       const uint64_t a_first = umma_desc_sw128(smem_u32(tiles)), b_first = umma_desc_sw128(smem_u32(tiles) + L8_A);
       const int mine = tile_first < tiles_all ? (tiles_all - tile_first + tile_step - 1) / tile_step : 0;
       const int turns = mine * k_blocks;
@@ -464,7 +465,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           ok = ok && mbar_wait(smem_u32(&sh.acc_empty[h][buf]), empty_parity, abort_flag);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t to = tmem_base + ((uint32_t)(h * ACC) + buf) * 128u;
+          const uint32_t to = tmem_base + ((uint32_t)(h * ACC) + buf) * (uint32_t)MMA_N;
 #pragma unroll
           for (int k = 0; k < L8_BK / 32; ++k) {      // 32 bytes further along the swizzled row: +2 in the 16-byte address field
             // (a pair's half: 64 weight rows of each block)
@@ -483,11 +484,13 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L8_REGS_ADD));
     constexpr int AHEAD = 4, WS = HALVES;
     const int quad = warp & 3, group = (warp - L8_FIRST) / 4, h = HALVES == 2 ? group : 0;
-    // column i of the warp's sums: weight row n0 + col0 + i / 64 * 128 + i % 64
-    const int col0 = group * 64;
-    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(HALVES == 2 ? h * ACC * 128 : group * 64);
+    // column i of the warp's sums: weight row n0 + col0 + i, or, of a pair's 256, n0 + col0 + i / 64 * 128 + i % 64
+    constexpr int SPAN = HALVES == 2 ? 64 : COLS, STRIDE = HALVES == 2 ? 128 : COLS;
+    const int col0 = group * SPAN;
+    const uint32_t from = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(HALVES == 2 ? h * ACC * 128 : group * COLS);
     const uint32_t full0 = smem_u32(&sh.acc_full[h][0]), empty0 = PAIR ? mapa_u32(smem_u32(&sh.acc_empty[h][0]), 0u) : smem_u32(&sh.acc_empty[h][0]);
-    const uint32_t staged = smem_u32(tiles) + (uint32_t)a.stages * STAGE + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
+    // (a block alone has one tile, and the ring is free behind its products)
+    const uint32_t staged = smem_u32(tiles) + (PAIR ? (uint32_t)a.stages * STAGE : 0u) + (uint32_t)(warp - L8_FIRST) * 2 * L8_BOX;
     float x_ahead[AHEAD], w_ahead[WS][AHEAD];
     const float *xs = a.xs, *ws = a.ws;
     bool has_x = false, has_w[WS];
@@ -498,6 +501,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       const int t = t0 + quad * 32 + lane;
       has_x = t < a.T;
       xs = a.xs + (size_t)k_first * a.T + (has_x ? t : 0);
+      if (!PAIR && SIDE_N == 256) n0 += col0;
       ws = a.ws + (size_t)(n0 / L8_BK) * a.blocks + k_first;
 #pragma unroll
       for (int i = 0; i < WS; ++i) has_w[i] = n0 + i * 128 < a.N;
@@ -522,7 +526,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         for (int d = 0; d < AHEAD; ++d) {
           const int kb = k0 + d;
           if (kb >= k_blocks || !ok) break;
-          const uint32_t buf = turn % ACC, at = from + buf * 128u;
+          const uint32_t buf = turn % ACC, at = from + buf * (uint32_t)MMA_N;
           float f[WS];
 #pragma unroll
           for (int i = 0; i < WS; ++i) f[i] = x_ahead[d] * w_ahead[i][d];
@@ -554,7 +558,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             }
             const uint32_t(&u)[16] = v[(c / 16) & 1];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) l8_fma2(acc[c / 2 + i], __uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), f[c / 64], f[c / 64]);
+            for (int i = 0; i < 8; ++i) l8_fma2(acc[c / 2 + i], __uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), f[c / SPAN], f[c / SPAN]);
           }
           ++turn;
         }
@@ -567,14 +571,14 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         for (int i = 0; i < COLS / 2; ++i) acc[i].x = acc[i].y = __int_as_float(L8_NONE);
       }
       const int row = quad * 32 + lane;
-      if (!PAIR && a.cut > 1) {
+      if (!PAIR && SIDE_N == 128 && a.cut > 1) {
         // all products are done, so the ring is free: this block's sums [128 tokens][128 + 4]
         if (ok) {
           float* part = reinterpret_cast<float*>(tiles) + row * (128 + 4) + col0;
 #pragma unroll
           for (int i = 0; i < COLS / 4; ++i) *reinterpret_cast<float4*>(part + 4 * i) = make_float4(acc[2 * i].x, acc[2 * i].y, acc[2 * i + 1].x, acc[2 * i + 1].y);
         }
-      } else if (boxes) {
+      } else if (boxes && (PAIR || ok)) {
         // 32 rows of 128 bytes at a time, laid out as the copy's swizzle has them; two boxes take turns
         constexpr int PER = 128 / (int)sizeof(O);
 #pragma unroll
@@ -601,7 +605,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            const int n = n0 + col0 + b * PER / 64 * 128 + b * PER % 64;
+            const int n = n0 + col0 + b * PER / SPAN * STRIDE + b * PER % SPAN;
             if (t0 + quad * 32 < a.T && n < a.N) l8_store_box(&tm_out, box, n, t0 + quad * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
@@ -611,7 +615,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         O* dst = out + (size_t)(t0 + row) * a.N;
 #pragma unroll
         for (int i = 0; i < COLS; ++i) {
-          const int n = n0 + col0 + i / 64 * 128 + i % 64;
+          const int n = n0 + col0 + i / SPAN * STRIDE + i % SPAN;
           if (n < a.N) dst[n] = qb_from_float<O>(i & 1 ? acc[i / 2].y : acc[i / 2].x);
         }
       }
@@ -620,7 +624,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (!PAIR && a.cut > 1) {
+  if (!PAIR && SIDE_N == 128 && a.cut > 1) {
     cluster_sync_all();
     // a share of the rows; without the parts of a block that gave up they are no numbers
     const bool missing = l8_missing(&sh.abort_flag, a.cut);
@@ -753,15 +757,18 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   if (a.blocks > 16)
     while (a.cut < 4 && singles * a.cut * 2 <= sms) a.cut *= 2;
   const bool pair = T > 128 && (singles > sms || (a.cut == 1 && a.blocks >= 32));
-  const int side = pair && singles > sms && waves_256 * 20 <= waves_128 * 13 ? 256 : 128, w_rows = pair && side == 128 ? 64 : 128;      // weight rows of a block's stage
+  // Up to 128 tokens: tiles of 256 weight rows, by the bytes of their waves (128 tokens, 4,096 x 22,016: 29.5 us in two waves of 128 rows, 23.6 in one).
+  const long long wide_waves = ((N + 255) / 256 + sms - 1) / sms, plain_waves = (singles + sms - 1) / sms;
+  const int side = (pair ? singles > sms && waves_256 * 20 <= waves_128 * 13 : T <= 128 && wide_waves * (128 + 256) < plain_waves * (128 + 128)) ? 256 : 128;
+  const int w_rows = pair ? side / 2 : side;      // weight rows of a block's stage
   const size_t size = out_dtype == QB_F32 ? 4 : 2;
   const int boxes = N * size % 16 == 0 && ((uintptr_t)out & 15) == 0;
   a.t_tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128);
   const long long tiles = (long long)((N + side - 1) / side) * a.t_tiles;
   a.per = (a.blocks + a.cut - 1) / a.cut;
   if (tiles * a.cut > 0x7fffffffll) return QB_ERR_UNSUPPORTED;
-  const size_t stage = L8_A + (size_t)w_rows * L8_BK, staged = a.cut > 1 ? 0 : 8 * 2 * L8_BOX;
-  a.stages = a.cut > 1 || w_rows == 64 ? 6 : 4;
+  const size_t stage = L8_A + (size_t)w_rows * L8_BK, staged = pair ? 8 * 2 * L8_BOX : 0;
+  a.stages = side == 128 ? 6 : 4;
   const size_t smem = stage * a.stages + staged + 1024;
   rc = l8_map(&tm_w, w, (uint64_t)N, (uint64_t)K, 1, (uint32_t)w_rows, bytes);
   if (!rc) rc = l8_map(&tm_x, x, (uint64_t)T, (uint64_t)K, 1, 128, bytes);
@@ -773,6 +780,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   QB_DISPATCH_DTYPE(out_dtype, O, {
     if (pair && side == 256) rc = l8_many<true, 256, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
     else if (pair) rc = l8_many<true, 128, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
+    else if (side == 256) rc = l8_many<false, 256, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
     else rc = l8_many<false, 128, O>(tm_w, tm_x, tm_out, a, boxes, grid, smem, stream);
   });
   if (rc) return rc;

@@ -328,7 +328,8 @@ LARGE_PRODUCTS = [(9, 4112, 9001), (16, 8192, 5000), (17, 4112, 4104), (32, 1100
                   (50, 65552, 129), (65, 16, 260000), (100, 4112, 1001), (128, 16400, 257), (129, 2064, 2085), (200, 5648, 2000), (257, 16, 5), (257, 144, 200),
                   (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500), (33, 8208, 2003), (64, 4240, 2000), (50, 65552, 300), (40, 144, 20001),
                   (128, 16400, 520), (257, 16, 4100), (300, 2192, 640), (260, 40016, 130), (700, 2320, 384), (1000, 512, 64), (9000, 16, 16), (5, 16, 40001),
-                  (400, 4112, 3000), (512, 5648, 4001), (1030, 4240, 2000), (1300, 4096, 4096), (200, 2064, 20008), (200, 2064, 20001)]      # pairs with 128 weight rows
+                  (400, 4112, 3000), (512, 5648, 4001), (1030, 4240, 2000), (1300, 4096, 4096), (200, 2064, 20008), (200, 2064, 20001),      # pairs with 128 weight rows
+                  (100, 2064, 22016), (128, 528, 20001), (70, 144, 37888), (65, 1040, 19080)]      # blocks alone with 256
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -361,7 +362,7 @@ def test_nan_stays_in_its_row_and_column_of_a_large_product(T, N):
     assert torch.equal(~torch.isfinite(out), want)
 
 
-@pytest.mark.parametrize("T,K,N", [(1, 512, 2048), (7, 4096, 700), (20, 2048, 1024), (40, 512, 512), (20, 8192, 4000), (64, 2048, 4096), (64, 4096, 2100), (100, 4096, 1024), (300, 512, 640), (300, 2048, 640)])
+@pytest.mark.parametrize("T,K,N", [(1, 512, 2048), (7, 4096, 700), (20, 2048, 1024), (40, 512, 512), (20, 8192, 4000), (64, 2048, 4096), (64, 4096, 2100), (100, 4096, 1024), (100, 512, 20000), (300, 512, 640), (300, 2048, 640)])
 def test_weights_read_ahead_of_the_rows(T, K, N):
     """Rows that the launch just before writes, in a chain, eagerly and in a graph: only the weights are read before it has ended."""
     from quanta_b200 import kernels
