@@ -6,7 +6,7 @@
 // many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the forms:
 //
 //  * 8 tokens or fewer, and more where the matrix is small: linear_fp8_few.cu, without tensor memory (its rule and both sides' times stand there).
-//  * up to 64 tokens (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
+//  * up to 32 tokens, or 64 (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
 //    height of the MMA and the weights are read once.  A TMEM lane is a weight row, a column a token; the columns' scales come from shared memory.
 //  * more (linear_fp8_kernel): the tokens are the rows, the weights the columns.  A lane has its token's scale in a register and one weight
 //    scale for all of its columns, so the addition is one packed multiply-add for two numbers and reads nothing.  (With the tokens as columns the
@@ -715,12 +715,15 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   a.status = status;
   const CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUtensorMap tm_w, tm_x, tm_out;
-  if (T <= 64) {
+  // Weights as rows up to 32 tokens, and up to 64 where they are cut along k (64 tokens, 8,192 x 8,192: 17.1 us, tokens as rows 18.6; 4,096 x 11,008, not
+  // cut as tokens' rows: 16.4 and 14.5).
+  const long long tiles_128 = (N + L8_M - 1) / L8_M;
+  if (T <= 32 || (T <= 64 && 2 * tiles_128 <= sms)) {
     const int NT = T <= 16 ? 16 : T <= 32 ? 32 : 64;
     a.t_tiles = 1;
-    const long long tiles = (N + L8_M - 1) / L8_M;
+    const long long tiles = tiles_128;
     // Along k as long as the parts are at most one an SM (a k block takes some 0.3 us, joining the parts some 2.5: 32 tokens, 16 tiles, 16 k blocks
-    // 8.4 us uncut, 5.7 in four parts, 5.9 in eight), and once more where a part is still long (86 tiles, 32 k blocks, 64 tokens: 19.7 us, 16.5 in two).
+    // 8.4 us uncut, 5.7 in four parts, 5.9 in eight), and once more where a part is still long (86 tiles, 32 k blocks, 32 tokens: 14.8 us, 14.0 in two).
     a.cut = 1;
     while (a.cut < 8 && tiles * a.cut * 2 <= sms && a.blocks >= (a.cut < 4 ? 8 : 32)) a.cut *= 2;
     if (a.cut < 8 && tiles * a.cut < sms && a.blocks / a.cut * NT >= 20 * 32) a.cut *= 2;
@@ -749,7 +752,7 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   // 128 takes some 0.65 of one of 256 (256 tokens, 4,096 x 22,016: 38 us in two waves of the one, 34.5 in three of the other; 1,024: 89 and 109).
   // Else single blocks, cut along k where they are few, or, where they are not cut and k is long, pairs with 128 rows, which fetch three quarters
   // of the bytes (512 tokens, 11,008 x 4,096: 35 and 30 us).
-  const long long singles = (long long)((T + 127) / 128) * ((N + 127) / 128), t_pairs = (T + 255) / 256;
+  const long long singles = (T + 127) / 128 * tiles_128, t_pairs = (T + 255) / 256;
   const long long waves_256 = (t_pairs * ((N + 255) / 256) * 2 + sms - 1) / sms, waves_128 = (t_pairs * ((N + 127) / 128) * 2 + sms - 1) / sms;
   // Along k where that saves more than the joining takes (256 tokens, 4,096 x 4,096, 32 k blocks: 15.3 us uncut, 12.3 in two parts; 16 k blocks and 32 tiles:
   // 8.1 us, 8.6 in four parts).

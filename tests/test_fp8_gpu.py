@@ -329,7 +329,8 @@ LARGE_PRODUCTS = [(9, 4112, 9001), (16, 8192, 5000), (17, 4112, 4104), (32, 1100
                   (300, 2064, 130), (260, 40016, 33), (1000, 144, 2600), (2049, 528, 1500), (33, 8208, 2003), (64, 4240, 2000), (50, 65552, 300), (40, 144, 20001),
                   (128, 16400, 520), (257, 16, 4100), (300, 2192, 640), (260, 40016, 130), (700, 2320, 384), (1000, 512, 64), (9000, 16, 16), (5, 16, 40001),
                   (400, 4112, 3000), (512, 5648, 4001), (1030, 4240, 2000), (1300, 4096, 4096), (200, 2064, 20008), (200, 2064, 20001),      # pairs with 128 weight rows
-                  (100, 2064, 22016), (128, 528, 20001), (70, 144, 37888), (65, 1040, 19080)]      # blocks alone with 256
+                  (100, 2064, 22016), (128, 528, 20001), (70, 144, 37888), (65, 1040, 19080),      # blocks alone with 256
+                  (64, 4112, 8200), (33, 4112, 9480), (64, 528, 11264), (50, 4096, 22016)]      # up to 64 tokens, as rows or as columns
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
