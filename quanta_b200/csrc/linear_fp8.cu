@@ -384,6 +384,15 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     l8_fetch_map(&tm_w);
     l8_fetch_map(&tm_x);
+    if (!PAIR && a.early) {      // a block alone: its first weights, as above
+      int n0, t0;
+      place(tile_first, n0, t0);
+      const uint64_t pol = l2_policy_evict_last();
+      for (int kb = 0; kb < min(a.stages, k_blocks); ++kb) {
+        mbar_expect_tx(smem_u32(&sh.full[kb]), STAGE);
+        tma_load_2d(smem_u32(tiles) + (uint32_t)kb * STAGE + L8_A, &tm_w, (k_first + kb) * L8_BK, n0, smem_u32(&sh.full[kb]), pol);
+      }
+    }
   }
   qb_follow();      // (no tensor memory before it: a block of the launch ahead may still have to get its own)
   if (warp == 1) {
@@ -421,20 +430,22 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           if (!ok) break;
           const uint32_t st = smem_u32(tiles) + (uint32_t)s * STAGE;
           // (a pair: every copy of either block counts on the first block's barrier, which expects both blocks' bytes)
-          if (rank == 0 || !PAIR) mbar_expect_tx(full0 + 8u * s, (PAIR ? 2 : 1) * STAGE);
+          const bool ahead = !PAIR && a.early && kb < a.stages;
+          if (!ahead && (rank == 0 || !PAIR)) mbar_expect_tx(full0 + 8u * s, (PAIR ? 2 : 1) * STAGE);
           if constexpr (PAIR) {
             tma_load_2d_pair(st, &tm_x, kb * L8_BK, t0, bars + 8u * s, pol);
             tma_load_2d_pair(st + L8_A, &tm_w, kb * L8_BK, n0, bars + 8u * s, pol);
           } else {
             tma_load_2d(st, &tm_x, (k_first + kb) * L8_BK, t0, full0 + 8u * s, pol);
-            tma_load_2d(st + L8_A, &tm_w, (k_first + kb) * L8_BK, n0, full0 + 8u * s, pol);
+            if (!ahead) tma_load_2d(st + L8_A, &tm_w, (k_first + kb) * L8_BK, n0, full0 + 8u * s, pol);
           }
           ++armed;
           if (++s == a.stages) { s = 0; parity ^= 1u; }
         }
       }
-      if (*abort_flag && PAIR && rank != 0) {
-        // this block's copies count on the other block's barriers, which it cannot wait on: give them time
+      const bool unarmed = !PAIR && a.early && armed < min(a.stages, k_blocks);
+      if (*abort_flag && ((PAIR && rank != 0) || unarmed)) {
+        // this block's copies count on the other block's barriers, which it cannot wait on, or on some that do not complete: give them time
         const uint64_t since = global_ns();
         for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
       } else if (*abort_flag) {
@@ -698,7 +709,7 @@ bool qb_linear_fp8_tokens_takes(int T, int K, int N);
 int qb_linear_fp8_tokens(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N, int early,
                          int sms, cudaStream_t stream);
 
-// early: w and ws were written two launches before this one at the latest (or by the host); the kernels for few tokens then ask for their
+// early: w and ws were written two launches before this one at the latest (or by the host); all but pairs of blocks then ask for their
 // first pieces before the launch ahead has ended.
 extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int T, int K, int N,
                              int early, int* status, cudaStream_t stream) {

@@ -1394,8 +1394,8 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     scale for every block of 128 x 128, ``[ceil(N / 128), ceil(K / 128)]``.  A block's products are summed by the tensor cores, the blocks
     scaled and summed in float32; ``out`` float32 or bfloat16 (one rounding).  K a multiple of 16; ``x`` and ``w`` on 16 bytes.  The same
     operands give the same bits in every run.  ``status``: where a bounded wait that ran out is recorded (the outputs are NaN then).
-    ``early``: nothing the two launches before this one do writes ``w`` or ``w_scales`` (the kernels for few tokens start to read them before
-    the launch before has ended)."""
+    ``early``: nothing the two launches before this one do writes ``w`` or ``w_scales`` (calls of few tokens start to read them before the launch
+    before has ended)."""
     _want(w, E4M3, "w"); _want(w_scales, torch.float32, "w_scales")
     if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
         raise ValueError("linear_fp8: x, w and out must be matrices")
