@@ -16,8 +16,9 @@
 //
 // Measured on a B200, one product after another in a graph: 8,192 tokens, 4,096 x 22,016 650 to 680 us (2.2 PFLOP/s; 775 where products follow one another
 // for seconds and the clock falls under the power limit), which is the power limit's and the issue's, the tensor cores being active 64% of the
-// cycles; 1,024 x 4,096 x 4,096 20 us; 317 x 5,648 x 2,000 16.6 us and 512 x 4,096 x 4,096 15 us, single blocks, which are bound by what an SM takes from
-// L2 (some 50 bytes a cycle; a 128 x 128 tile reads 256 bytes for every 128 x 128 products); 32 tokens, 4,096 x 11,008 14 us, the bytes 7.
+// cycles; 1,024 x 4,096 x 4,096 20 us; 512 x 4,096 x 4,096 14.7 us and, in two parts along k, 317 x 5,648 x 2,000 16.2 us, which are bound by what an SM takes
+// from L2 (some 50 bytes a cycle; a 128 x 128 tile reads 256 bytes for every 128 x 128 products); 128 x 4,096 x 22,016 23.7 us, the bytes 14; 32 x 11,008 x 4,096
+// 13.4 us, the bytes 7.
 //
 // A product of few tiles is cut along k over the blocks of a cluster; each leaves its sums in shared memory, and every block adds one share of
 // them, the blocks' parts in order, so the result is the same in every run.
