@@ -41,28 +41,39 @@ __device__ __forceinline__ void fp8_no_row(const NormFp8& a, int r) {
   }
 }
 
-// x += the slots' eight numbers from column i on, slots in order
-template <typename D>
+// A thread's eight numbers of a row: eight neighbours from column i on, or (rows of no whole, aligned pieces) every sixteenth of a block from i on, of
+// which `left` exist, 16 apart.
+template <bool VEC, typename D>
+__device__ __forceinline__ void fp8_load8(const D* row, int i, int left, float (&v)[8]) {
+  if constexpr (VEC) {
+    QbVec8<D>::load(row + i, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e * 16 < left ? qb_to_float<D>(row[i + e * 16]) : 0.f;
+  }
+}
+// x += the slots' eight numbers, slots in order
+template <bool VEC, typename D>
 __device__ __forceinline__ void fp8_add_slots(const NormFp8& a, int tok, int i, float (&x)[8]) {
-  const D* d = (const D*)a.delta + (size_t)tok * a.S * a.H + i;
+  const D* d = (const D*)a.delta + (size_t)tok * a.S * a.H;
 #pragma unroll 2
   for (int s = 0; s < a.S; ++s) {
     float dv[8];
-    QbVec8<D>::load(d + (size_t)s * a.H, dv);
+    fp8_load8<VEC, D>(d + (size_t)s * a.H, i, a.H - i, dv);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] += dv[e];
   }
 }
 
-// Rows of whole 32-byte pieces of at most 8,192 numbers: a thread keeps its 8 in registers from the load to the store, 16 threads hold a block
-// of 128 and find its largest among themselves.
+// Rows of at most 8,192 numbers: a thread keeps its 8 in registers from the load to the store, 16 threads hold a block of 128 and find its largest
+// among themselves.  VEC: rows of whole 32-byte pieces.
 // MOST: threads at most.  Without a gain the registers are held down to 32, so that an SM has the bytes of four rows on their way (8,192 rows of 4,096,
 // two float32 slots: 97 us with 40, 88 with 32; with a gain, and 40 instead of 56, they spill: 45 -> 59 us at 2,048).
-template <typename D, bool GAIN, int MOST>
-__global__ void __launch_bounds__(MOST, GAIN && MOST == 1024 ? 1 : 2) norm_fp8_rows_kernel(NormFp8 a) {
+template <typename D, bool GAIN, int MOST, bool VEC>
+__global__ void __launch_bounds__(MOST, (GAIN || !VEC) && MOST == 1024 ? 1 : 2) norm_fp8_rows_kernel(NormFp8 a) {
   qb_follow();
   __shared__ float scratch[2][32];
-  const int r = blockIdx.x, tok = a.rows != nullptr ? a.rows[r] : r, i = threadIdx.x * 8;
+  const int r = blockIdx.x, tok = a.rows != nullptr ? a.rows[r] : r, i = VEC ? threadIdx.x * 8 : threadIdx.x / 16 * FP8_BLOCK + threadIdx.x % 16;
   const bool in = i < a.H;
   if (tok < 0 || tok >= a.T) {
     fp8_no_row(a, r);
@@ -76,9 +87,9 @@ __global__ void __launch_bounds__(MOST, GAIN && MOST == 1024 ? 1 : 2) norm_fp8_r
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = w[e] = 0.f;
     if (in) {
-      QbVec8<float>::load(a.h + (size_t)tok * a.H + i, x);
-      QbVec8<float>::load(a.g + i, w);
-      fp8_add_slots<D>(a, tok, i, z);
+      fp8_load8<VEC, float>(a.h + (size_t)tok * a.H, i, a.H - i, x);
+      fp8_load8<VEC, float>(a.g, i, a.H - i, w);
+      fp8_add_slots<VEC, D>(a, tok, i, z);
     }
     float ss = 0.f;
 #pragma unroll
@@ -87,27 +98,43 @@ __global__ void __launch_bounds__(MOST, GAIN && MOST == 1024 ? 1 : 2) norm_fp8_r
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] += w[e] * (z[e] * inv);
   } else if (in) {
-    QbVec8<float>::load(a.h + (size_t)tok * a.H + i, x);
-    if (a.delta != nullptr) fp8_add_slots<D>(a, tok, i, x);
+    fp8_load8<VEC, float>(a.h + (size_t)tok * a.H, i, a.H - i, x);
+    if (a.delta != nullptr) fp8_add_slots<VEC, D>(a, tok, i, x);
   }
   float ss = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-  if (in && a.store_h && a.delta != nullptr) QbVec8<float>::store(a.h + (size_t)tok * a.H + i, x);
+  if (in && a.store_h && a.delta != nullptr) {
+    float* h = a.h + (size_t)tok * a.H + i;
+    if constexpr (VEC) {
+      QbVec8<float>::store(h, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e * 16 < a.H) h[e * 16] = x[e];
+    }
+  }
   // the gains are every block's, so they are near; asked for before the sum
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = 0.f;
-  if (in) QbVec8<float>::load(a.w + i, w);
+  if (in) fp8_load8<VEC, float>(a.w, i, a.H - i, w);
   const float inv = rsqrtf(fp8_row_sum(ss, scratch[1]) / (float)a.H + a.eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = w[e] * (x[e] * inv);
   const float top = fp8_block_largest(fp8_largest(x));
   if (!in) return;
-  *reinterpret_cast<uint2*>(a.out + (size_t)r * a.H + i) = fp8_eight(x, fp8_up(top));
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2*>(a.out + (size_t)r * a.H + i) = fp8_eight(x, fp8_up(top));
+  } else {
+    const float up = fp8_up(top);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e * 16 < a.H) a.out[(size_t)r * a.H + i + e * 16] = fp8_one(x[e] * up);
+  }
   if ((threadIdx.x & 15) == 0) a.scales[(size_t)(i / FP8_BLOCK) * a.n + r] = fp8_scale(top);
 }
 
-// Any other row: held in shared memory between the passes, a warp a block of 128.
+// Longer rows: held in shared memory between the passes, a warp a block of 128.
 template <typename D>
 __global__ void __launch_bounds__(512) norm_fp8_any_kernel(NormFp8 a) {
   extern __shared__ float row[];      // H floats
@@ -320,12 +347,15 @@ extern "C" int qb_add_rmsnorm_fp8(float* h, const void* delta, int delta_dtype, 
   if (n_rows <= 0 || H <= 0) return 0;
   if (g != nullptr && delta == nullptr) return QB_ERR_BAD_ARG;
   const NormFp8 a{h, delta, w, g, (uint8_t*)out, scales, rows, S, n_rows, T, H, eps, eps_d, store_h};
-  if (H % 8 == 0 && H <= 8192 && (((uintptr_t)h | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)g) & 15) == 0 && ((uintptr_t)out & 7) == 0) {
-    const int threads = (H / 8 + 31) / 32 * 32;
+  if (H <= 8192) {
+    const bool vec = H % 8 == 0 && (((uintptr_t)h | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)g) & 15) == 0 && ((uintptr_t)out & 7) == 0;
+    const int threads = ((H + FP8_BLOCK - 1) / FP8_BLOCK * 16 + 31) / 32 * 32;
     QB_DISPATCH_DTYPE(delta_dtype, D, {
-      if (g != nullptr && threads <= 512) qb_launch(norm_fp8_rows_kernel<D, true, 512>, n_rows, threads, 0, stream, a);
-      else if (g != nullptr) qb_launch(norm_fp8_rows_kernel<D, true, 1024>, n_rows, threads, 0, stream, a);
-      else qb_launch(norm_fp8_rows_kernel<D, false, 1024>, n_rows, threads, 0, stream, a);
+      if (!vec && g != nullptr) qb_launch(norm_fp8_rows_kernel<D, true, 1024, false>, n_rows, threads, 0, stream, a);
+      else if (!vec) qb_launch(norm_fp8_rows_kernel<D, false, 1024, false>, n_rows, threads, 0, stream, a);
+      else if (g != nullptr && threads <= 512) qb_launch(norm_fp8_rows_kernel<D, true, 512, true>, n_rows, threads, 0, stream, a);
+      else if (g != nullptr) qb_launch(norm_fp8_rows_kernel<D, true, 1024, true>, n_rows, threads, 0, stream, a);
+      else qb_launch(norm_fp8_rows_kernel<D, false, 1024, true>, n_rows, threads, 0, stream, a);
     });
     QB_LAUNCH_CHECK();
     return 0;

@@ -477,3 +477,42 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+ODD_NORMS = [(3, 2434, 1), (50, 1062, 8), (300, 789, 1), (4, 8191, 2), (2, 129, 1), (1000, 33, 3), (2, 8193, 1)]
+
+
+@pytest.mark.parametrize("gain", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,H,S", ODD_NORMS)
+def test_norm_of_rows_that_do_not_lie_on_16_bytes(n, H, S, dtype, gain):
+    test_norm(n, H, S, dtype, gain)
+
+
+def test_rows_of_any_place():
+    """Rows that begin one number behind a 16-byte place, of a width that would be whole pieces: the same numbers as rows that do not."""
+    from quanta_b200 import kernels
+    g = _gen(12)
+    n, H = 9, 1024
+    h, d, w = _randn(g, n, H), _randn(g, n, H), 1 + 0.2 * _randn(g, H)
+    q, s = _empty_rows(n, H)
+    h0 = h.clone()
+    kernels.add_rmsnorm_fp8(h0, d, w, 1e-5, q, s)
+    behind = lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)  # noqa: E731
+    h1, q1, s1 = behind(h), behind(q.view(torch.uint8)).view(E4M3), torch.empty_like(s)
+    kernels.add_rmsnorm_fp8(h1, behind(d), behind(w), 1e-5, q1, s1)
+    assert torch.equal(h1, h0)
+    # (the sums of squares are taken in another order)
+    assert torch.all((q1.float() * _spread(s1, H) - q.float() * _spread(s, H)).abs() <= 2.0 ** -4 * (q.float() * _spread(s, H)).abs() + 2.0 ** -9 * _spread(s, H))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N", [(1054, 1280, 3207), (300, 144, 20003), (2000, 528, 1999), (128, 528, 20003), (100, 4112, 1003), (40, 8208, 2001), (130, 2064, 2086), (700, 4112, 4095)])
+def test_product_whose_rows_do_not_lie_on_16_bytes(T, K, N, dtype):
+    from quanta_b200 import kernels
+    ops = _operands(T, K, N, T + K + N)
+    big = torch.full((T * N + 512,), 7.0, device=DEV, dtype=dtype)
+    out = big[256: 256 + T * N].view(T, N)
+    kernels.linear_fp8(*ops, out)
+    assert torch.all(big[:256] == 7) and torch.all(big[256 + T * N:] == 7)
+    _product_within(out, *ops)
