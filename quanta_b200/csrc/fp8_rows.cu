@@ -1,7 +1,7 @@
 // Rows that leave a norm, an activation or another kernel in e4m3 with a scale for every 128 columns (fp8.cuh): what a product in 8 bits reads.
 //
 // All of them are bound by memory; what 8 bits save is that the row passes it once, with one byte a number on the way out.  Measured on a B200, one
-// after another in a graph: norm of 8,192 x 4,096 with two float32 slots 88 us (6.4 TB/s), one row 2.4 us; activation of 8,192 x 11,008 bfloat16, clamped with
+// after another in a graph: norm of 8,192 x 4,096 with two float32 slots 88 us (6.4 TB/s), one row 2.4 us, of 6,311 x 2,434 (rows that do not lie on 16 bytes) with a bfloat16 addend 34 us (5.0 TB/s); activation of 8,192 x 11,008 bfloat16, clamped with
 // biases 82 us (5.5 TB/s), silu without 70 (6.5 TB/s), one row 1.6 us.
 #include "fp8.cuh"
 
@@ -243,7 +243,8 @@ __device__ __forceinline__ float2 act_two(float2 g, float2 u, float limit, float
 
 // Sixteen threads hold a block of 128 columns, eight numbers each, and take the same columns of neighbouring rows: the biases stay in registers,
 // the numbers of several rows (128 bytes a thread) are on their way together, and the rows' scales of a block are neighbours.  VEC: whole 16-byte
-// pieces; else neighbouring threads take neighbouring numbers of the block.
+// pieces; else neighbouring threads take neighbouring numbers of the block (8,192 x 11,007 bfloat16, silu 113 us, 69 on whole pieces; two or four rows on
+// their way 118 and 170).
 constexpr int ACT_THREADS = 256, ACT_COLS = ACT_THREADS * 8, ACT_ROWS = 8;
 template <typename T, int KIND, bool BIAS, bool VEC>
 __global__ void __launch_bounds__(ACT_THREADS) act_fp8_kernel(ActFp8 a, int rows_each) {
@@ -292,12 +293,22 @@ __global__ void __launch_bounds__(ACT_THREADS) act_fp8_kernel(ActFp8 a, int rows
         QbVec8<T>::load(reinterpret_cast<const T*>(raw[d][0]), g);
         QbVec8<T>::load(reinterpret_cast<const T*>(raw[d][1]), u);
       } else {
+        // (all are asked for before the first is looked at)
         const T* row = (const T*)a.x + (size_t)r * width;
+        T one[2][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int i = column(e);
-          g[e] = i < a.I ? qb_to_float<T>(row[i]) : 0.f;
-          u[e] = KIND != ACT_NONE && i < a.I ? qb_to_float<T>(row[a.I + i]) : 0.f;
+          one[0][e] = one[1][e] = qb_from_float<T>(0.f);
+          if (i < a.I) {
+            one[0][e] = row[i];
+            if (KIND != ACT_NONE) one[1][e] = row[a.I + i];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          g[e] = qb_to_float<T>(one[0][e]);
+          u[e] = qb_to_float<T>(one[1][e]);
         }
       }
 #pragma unroll
