@@ -24,7 +24,9 @@
 // them, the blocks' parts in order, so the result is the same in every run.
 //
 // Every wait on an mbarrier is bounded; when one runs out the block records it in the status words, its outputs are NaN, it lets its copies in
-// flight land, frees its TMEM and returns.
+// flight land, frees its TMEM and returns.  The wait for tensor memory (tcgen05.alloc) has no bound, so nothing that holds tensor memory waits for another block:
+// it is given back before the cluster's barriers.  A pair's blocks do wait for one another with it, but where they ask for it nobody else can have it:
+// they take an SM's registers (64,512 of 65,536) for themselves.
 #include "fp8.cuh"
 #include "tensor_core.cuh"
 
@@ -319,6 +321,13 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  // Given back before the cluster's barriers: a block that still waits for tensor memory reaches them only once it has some, and those it waits
+  // for may be of its own cluster, or of another that holds columns here and waits for them on another SM (at 64 tokens, 1,024 x 4,096, shared memory
+  // places four blocks on an SM, tensor memory two).
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
+  }
   if (a.cut > 1) {
     cluster_sync_all();
     // a share of the columns; without the parts of a block that gave up it is no number
@@ -332,7 +341,6 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     cluster_sync_all();      // the parts stay until all have read them
   }
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
   if (threadIdx.x == 0 && sh.abort_flag) qb_set_status(a.status, QB_STATUS_WAIT_TIMEOUT, tile, 11);
 }
 
@@ -671,6 +679,12 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (!PAIR) {      // before the cluster's barriers, as above
+    if (warp == 1) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
+    }
+  }
   if (!PAIR && SIDE_N == 128 && a.cut > 1) {
     cluster_sync_all();
     // a share of the rows; without the parts of a block that gave up they are no numbers
@@ -686,11 +700,11 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       l8_store4(out + (size_t)(t0 + row) * a.N, n0 + col, a.N, sum);
     }
   }
-  // no block leaves, or gives its accumulators back, while another's MMAs or sums may read what it has
+  // no block leaves while another reads its parts, and none of a pair, whose blocks have got their tensor memory together, gives it back while the other's
+  // MMAs or sums may use it
   if (PAIR || a.cut > 1) cluster_sync_all();
-  if (warp == 1) {
-    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
+  if constexpr (PAIR) {
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
   }
   if (threadIdx.x == 0 && sh.abort_flag) qb_set_status(a.status, QB_STATUS_WAIT_TIMEOUT, tile_first, 11);
 }
