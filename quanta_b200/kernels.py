@@ -1259,6 +1259,7 @@ def glu_act(gate_up: torch.Tensor, out: torch.Tensor, *, bias=None, kind: int = 
 FP8_BLOCK = 128                 # columns of a row, and rows and columns of a weight, that share a scale
 E4M3 = torch.float8_e4m3fn
 MOST_ROWS = 1 << 30             # rows, and columns of a row: the kernels count them, and what they take together, in 32 bits
+FP8_NORM_MAX_WIDTH = 51200      # rows of a norm wider than 8,192 are held in shared memory (200 KB) between its passes
 
 
 _VOID, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
@@ -1322,11 +1323,14 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: torch.Tensor | None, weight: torch.T
     float8_e4m3fn, ``scales`` ``[ceil(H / 128), n]``, the numbers they stand for ``out[r, c] * scales[c // 128, r]``.  A scale is the
     block's largest number / 448, at least 2^-100 / 448.  ``delta`` (``[T, H]`` or ``[T, S, H]``, float32 or bfloat16, or None) is summed
     over its slots; with ``delta_gain`` (float32 ``[H]``) it is normed first, ``delta_gain * d * rsqrt(mean(d^2) + delta_eps)``.
-    ``rows`` (int32) selects token rows, which needs ``store_h`` False (a row may be selected twice); one outside ``h`` gives NaN."""
+    ``rows`` (int32) selects token rows, which needs ``store_h`` False (a row may be selected twice); one outside ``h`` gives NaN.  H is at most
+    ``FP8_NORM_MAX_WIDTH``."""
     _want(h, torch.float32, "h"); _want(weight, torch.float32, "weight")
     if h.dim() != 2:
         raise ValueError("add_rmsnorm_fp8: h must be [T, H]")
     T, H = h.shape
+    if H > FP8_NORM_MAX_WIDTH:
+        raise ValueError(f"add_rmsnorm_fp8: rows of at most {FP8_NORM_MAX_WIDTH} numbers are taken, got {H}")
     S = 1
     if delta is not None:
         shape = delta.shape
