@@ -375,7 +375,7 @@ extern "C" int qb_add_rmsnorm_fp8(float* h, const void* delta, int delta_dtype, 
   if (smem > 200 * 1024) return QB_ERR_UNSUPPORTED;
   QB_DISPATCH_DTYPE(delta_dtype, D, {
     auto kern = norm_fp8_any_kernel<D>;
-    if (smem > 48 * 1024) {
+    if (smem + 1024 > 48 * 1024) {      // (the kernel also has some static shared memory)
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return (int)e;
     }

@@ -51,3 +51,11 @@ def test_selected_rows_and_no_addend(H):
         bad = [0, 2, 3]
         assert torch.equal(h3, h) and torch.all(torch.isnan(q3.float()[bad])) and torch.all(torch.isnan(s3[:, bad]))
         assert torch.equal(q3.float()[1], full.float()[2]) and torch.equal(s3[:, 1], full_s[:, 2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [12032, 12033, 12224, 12225, 12256, 12288, 12289])
+def test_rows_that_fill_what_shared_memory_a_kernel_has_unasked(H, dtype):
+    """48 KB, of which the kernel's own variables take some: a row that leaves no room for them has to ask for more."""
+    _norm_within(3, H, 1, dtype, False)
