@@ -630,7 +630,7 @@ extern "C" int qb_streams_mix_rmsnorm(float* x, int S, const void* delta, int de
 #define QB_STREAMS(SS_)                                                                                          \
   do {                                                                                                           \
     auto kern = streams_mix_rmsnorm_kernel<D, O, SS_>;                                                           \
-    if (smem > 48 * 1024) {                                                                                      \
+    if (smem + 2048 > 48 * 1024) {   /* the kernel also has some static shared memory */                         \
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);        \
       if (e != cudaSuccess) return (int)e;                                                                       \
     }                                                                                                            \

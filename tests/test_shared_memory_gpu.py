@@ -1,0 +1,14 @@
+"""Rows that fill the 48 KB of shared memory that a kernel has unasked, but for what its own variables take: it has to ask for more."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_tirizen_gpu import test_streams_between_two_sublayers_in_one_launch as _streams
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("S,width,K", [(1, 11968, 1), (2, 11969, 1), (3, 12000, 2), (2, 12256, 1), (1, 12288, 1)])
+def test_norm_over_several_streams(S, width, K):
+    _streams(S, width, K)
