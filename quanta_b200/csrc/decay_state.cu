@@ -1099,7 +1099,7 @@ extern "C" int qb_decay_out(const float* o, const float* den, const void* x, lon
 #define DS_OUT(WARPS, Q)                                                                                              \
   do {                                                                                                               \
     auto kern = decay_out_kernel<O, WARPS, Q>;                                                                        \
-    if (smem > 48 * 1024) {                                                                                           \
+    if (smem + 1024 > 48 * 1024) {   /* the kernel also has some static shared memory */                              \
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);              \
       if (e != cudaSuccess) return (int)e;                                                                            \
     }                                                                                                                 \
