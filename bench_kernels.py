@@ -5,6 +5,7 @@
     python bench_kernels.py attn_sweep                      # the cases quoted under profiles/
     python bench_kernels.py router       --tokens 2048      # router logits + selection of a prompt portion
     python bench_kernels.py experts      --tokens 8         # routed experts of one layer: plan, gather, two products
+    python bench_kernels.py feed_forward --tokens 8 --hidden 4096 --width 11008      # a norm and a gated feed-forward, in bfloat16 and in 8 bits
 
 Shapes default to the M2-family attention (48 q heads, 8 kv heads of 128, pages of 16 tokens).  Caches
 are random, pages are dealt in a random order, every request of a decode case has the same context.
@@ -205,9 +206,50 @@ def experts(tokens: int, hidden: int, width: int, n_experts: int, top_k: int, ev
     return out
 
 
+def feed_forward(tokens: int, hidden: int, width: int) -> dict:
+    """A norm and the gated feed-forward behind it (``GatedDense``, silu) as a model runs them, with matrices in bfloat16 and held in 8 bits, launches in
+    a CUDA graph, the two in turn; four sets of weights in turn, so that a step of few tokens finds none of them in L2.  ``rows_us``: rows of the
+    activation dtype brought to 8 bits, which blocks whose norm is also read by others do instead."""
+    from types import SimpleNamespace
+
+    from quanta_b200 import fp8, matmul
+    from quanta_b200.parts.dense import GatedDense
+    from quanta_b200.parts.norms import RMSNorm, rows_for
+    matmul.configure()
+    ctx = SimpleNamespace(dtype=torch.bfloat16, settled=True, status=k.new_status(DEV))
+    norm = RMSNorm(hidden, 1e-5, "norm")
+    norm.weight = torch.ones(hidden, device=DEV)
+    h, y = torch.randn(tokens, hidden, device=DEV), torch.randn(tokens, hidden, device=DEV)
+    parts = {"bf16": [], "fp8": []}
+    for i in range(4):
+        w = {n: torch.empty(shape, device=DEV, dtype=torch.bfloat16).normal_(0, 0.02)
+             for n, shape in (("gate", (width, hidden)), ("up", (width, hidden)), ("down", (hidden, width)))}
+        for held in parts.values():
+            held.append(GatedDense(hidden, width, {n: n for n in w}))
+            held[-1].load(w.get)
+        parts["fp8"][-1].hold_in_fp8()
+
+    def run(held):
+        for part in held:
+            x = rows_for(part, norm, h, hidden, torch.bfloat16)
+            norm.forward(h, y, x, store_h=False)
+            part.forward(x, ctx)
+
+    times = {name: [] for name in parts}
+    for _ in range(5):
+        for name, held in parts.items():
+            times[name].append(timed_graph(lambda held=held: run(held), reps=2) / 4 * 1e3)
+    x = torch.randn(tokens, hidden, device=DEV).bfloat16()
+    out = {"kernel": "norm + gated feed-forward", "tokens": tokens, "hidden": hidden, "width": width}
+    out.update({f"{name}_us": round(sorted(t)[2], 1) for name, t in times.items()})
+    out["rows_us"] = round(timed_graph(lambda: fp8.quantize_rows(x)) * 1e3, 1)
+    assert int(ctx.status[0]) == 0
+    return out
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("what", choices=["attn_decode", "attn_span", "attn_sweep", "router", "experts"])
+    ap.add_argument("what", choices=["attn_decode", "attn_span", "attn_sweep", "router", "experts", "feed_forward"])
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--context", type=int, default=4096)
     ap.add_argument("--tokens", type=int, default=2048)
@@ -219,7 +261,7 @@ def main() -> None:
     ap.add_argument("--hidden", type=int, default=3072)
     ap.add_argument("--experts", type=int, default=256)
     ap.add_argument("--top-k", type=int, default=8)
-    ap.add_argument("--width", type=int, default=1536, help="inner size of an expert")
+    ap.add_argument("--width", type=int, default=1536, help="inner size of an expert, or of the feed-forward")
     ap.add_argument("--even-routing", action="store_true", help="experts: the same number of rows for every expert")
     a = ap.parse_args()
     shape = (a.q_heads, a.kv_heads, a.head_dim, a.page)
@@ -229,6 +271,8 @@ def main() -> None:
         print(json.dumps(attn_span(a.tokens, a.start, *shape)), flush=True)
     elif a.what == "experts":
         print(json.dumps(experts(a.tokens, a.hidden, a.width, a.experts, a.top_k, a.even_routing)), flush=True)
+    elif a.what == "feed_forward":
+        print(json.dumps(feed_forward(a.tokens, a.hidden, a.width)), flush=True)
     elif a.what == "router":
         print(json.dumps(router(a.tokens, a.hidden, a.experts, a.top_k)), flush=True)
     else:
