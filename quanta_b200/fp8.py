@@ -28,10 +28,6 @@ class Fp8Rows:
     def shape(self):
         return self.q.shape
 
-    def dequantized(self) -> torch.Tensor:
-        """The numbers they stand for, float32 (for tools; the kernels read the rows as they are)."""
-        return self.q.float() * self.scales.t().repeat_interleave(BLOCK, 1)[:, : self.q.shape[1]]
-
 
 @dataclass(frozen=True)
 class Fp8Weight:
@@ -44,6 +40,7 @@ class Fp8Weight:
         return self.q.shape
 
     def dequantized(self) -> torch.Tensor:
+        """The numbers it stands for, float32 (for tools; the kernels read the matrix as it is)."""
         n, k = self.q.shape
         return self.q.float() * self.scales.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
 
