@@ -1,7 +1,8 @@
 // Rows that leave a norm, an activation or another kernel in e4m3 with a scale for every 128 columns (fp8.cuh): what a product in 8 bits reads.
 //
 // All of them are bound by memory; what 8 bits save is that the row passes it once, with one byte a number on the way out.  Measured on a B200, one
-// after another in a graph: norm of 8,192 x 4,096 with two float32 slots 88 us (6.4 TB/s), one row 2.4 us, of 6,311 x 2,434 (rows that do not lie on 16 bytes) with a bfloat16 addend 34 us (5.0 TB/s); activation of 8,192 x 11,008 bfloat16, clamped with
+// after another in a graph: norm of 8,192 x 4,096 with two float32 slots 88 us (6.5 TB/s), one row 2.4 us, of 6,311 x 2,434 (rows that do not lie on 16 bytes) with a bfloat16 addend 34 us (5.0 TB/s);
+// plain rows of 8,192 x 11,008 bfloat16 42 us (6.5 TB/s), one row 1.3 us; activation of 8,192 x 11,008 bfloat16, clamped with
 // biases 82 us (5.5 TB/s), silu without 70 (6.5 TB/s), one row 1.6 us.
 #include "fp8.cuh"
 
@@ -134,7 +135,8 @@ __global__ void __launch_bounds__(MOST, (GAIN || !VEC) && MOST == 1024 ? 1 : 2) 
   if ((threadIdx.x & 15) == 0) a.scales[(size_t)(i / FP8_BLOCK) * a.n + r] = fp8_scale(top);
 }
 
-// Longer rows: held in shared memory between the passes, a warp a block of 128.
+// Longer rows: held in shared memory between the passes, a warp a block of 128.  Number by number, so some 2.3 times the bytes' time (one float32
+// addend, 4,096 x 12,288: 233 us, the bytes 100; 2,048 x 20,000: 249 and 81; one row of 8,200 9.4 us): no model here is as wide.
 template <typename D>
 __global__ void __launch_bounds__(512) norm_fp8_any_kernel(NormFp8 a) {
   extern __shared__ float row[];      // H floats
@@ -212,7 +214,8 @@ __device__ __forceinline__ float fp8_min(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// The exponential and the reciprocal are the fast ones (some 2 ulp, and 2^-23 of the argument): what follows is rounded to four bits.
+// The exponential and the reciprocal are the fast ones (some 2 ulp, and 2^-23 of the argument; a sigmoid below 2^-126 is zero): what follows is rounded to
+// four bits.
 __device__ __forceinline__ float2 fp8_sigmoid2(float2 g, float by) {      // 1 / (1 + e^(-g by / log2 e))
   const float2 z = fp8_mul2(g, make_float2(-by, -by));
   float2 e;
@@ -244,7 +247,8 @@ __device__ __forceinline__ float2 act_two(float2 g, float2 u, float limit, float
 // Sixteen threads hold a block of 128 columns, eight numbers each, and take the same columns of neighbouring rows: the biases stay in registers,
 // the numbers of several rows (128 bytes a thread) are on their way together, and the rows' scales of a block are neighbours.  VEC: whole 16-byte
 // pieces; else neighbouring threads take neighbouring numbers of the block (8,192 x 11,007 bfloat16, silu 113 us, 69 on whole pieces; two or four rows on
-// their way 118 and 170).
+// their way 118 and 170).  A block spans 2,048 columns, so in narrower rows threads have nothing to do (8,192 rows bfloat16, silu: 512 columns 14.5 us, the
+// bytes 3.2; 1,408 15.5 and 8.8; 2,056 21.3 and 12.9; plain rows of 512 9.4 and 1.9).
 constexpr int ACT_THREADS = 256, ACT_COLS = ACT_THREADS * 8, ACT_ROWS = 8;
 template <typename T, int KIND, bool BIAS, bool VEC>
 __global__ void __launch_bounds__(ACT_THREADS) act_fp8_kernel(ActFp8 a, int rows_each) {

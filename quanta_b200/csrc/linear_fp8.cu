@@ -5,8 +5,9 @@
 // (one rounding a block); several accumulators take turns, so that the tensor cores work on the next block meanwhile.  That addition has as
 // many elements as the tile and has to keep up with the products (512 cycles for 128 x 256 and 128 k), which decides the forms:
 //
-//  * 8 tokens or fewer, and more where the matrix is small: linear_fp8_few.cu, without tensor memory (its rule and both sides' times stand there).
-//  * up to 32 tokens, or 64 (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
+//  * 8 tokens or fewer, but for matrices of very many short rows, and more where the matrix is small: linear_fp8_few.cu, without tensor memory (its
+//    rule and both sides' times stand there).
+//  * up to 32 tokens, or 64 of a matrix of few rows (linear_fp8_few_kernel): the weights are the 128-row operand and the tokens the N operand, so that few tokens use the full
 //    height of the MMA and the weights are read once.  A TMEM lane is a weight row, a column a token; the columns' scales come from shared memory.
 //  * more (linear_fp8_kernel): the tokens are the rows, the weights the columns.  A lane has its token's scale in a register and one weight
 //    scale for all of its columns, so the addition is one packed multiply-add for two numbers and reads nothing.  (With the tokens as columns the
@@ -776,8 +777,9 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
   a.status = status;
   const CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUtensorMap tm_w, tm_x, tm_out;
-  // Weights as rows up to 32 tokens, and up to 64 where they are cut along k (64 tokens, 8,192 x 8,192: 17.1 us, tokens as rows 18.6; 4,096 x 11,008, not
-  // cut as tokens' rows: 16.4 and 14.5).
+  // Weights as rows up to 32 tokens, and up to 64 where their tiles are half the SMs at most, so that eight k blocks and more are cut along k (64 tokens,
+  // 8,192 x 8,192: 19.2 us, tokens as rows 20.1; 4,096 x 4,096: 9.7 and 10.2; 4,096 x 11,008, 86 tiles: 16.9 and 14.6).  With a short k that is the slower
+  // side (64 tokens, 512 x 8,000, uncut: 5.9 and 5.0; 1,024 x 5,000, in two parts: 7.1 and 5.8; 2,048 x 9,000: 9.8 and 9.0).
   const long long tiles_128 = (N + L8_M - 1) / L8_M;
   if (T <= 32 || (T <= 64 && 2 * tiles_128 <= sms)) {
     const int NT = T <= 16 ? 16 : T <= 32 ? 32 : 64;
@@ -808,15 +810,15 @@ extern "C" int qb_linear_fp8(const void* x, const float* xs, const void* w, cons
     QB_LAUNCH_CHECK();
     return 0;
   }
-  // Pairs of blocks where tiles of 128 x 128 would be more than one for every SM (768 tokens, 4,096 x 4,096: 20 us, 29 with single blocks; 512, one tile an
-  // SM: 19 and 15), but for tokens that fill half a pair's tile at most.  256 weight rows a pair or 128, whichever makes the shorter waves: a tile of
-  // 128 takes some 0.65 of one of 256 (256 tokens, 4,096 x 22,016: 38 us in two waves of the one, 34.5 in three of the other; 1,024: 89 and 109).
+  // Pairs of blocks where tiles of 128 x 128 would be more than one for every SM (768 tokens, 4,096 x 4,096: 21 us, 27 with single blocks; 512, one tile an
+  // SM: 19 and 14), but for tokens that fill half a pair's tile at most.  256 weight rows a pair or 128, whichever makes the shorter waves: a tile of
+  // 128 takes some 0.65 of one of 256 (256 tokens, 4,096 x 22,016: 39 us in two waves of the one, 35 in three of the other; 1,024: 92 and 115).
   // Else single blocks, cut along k where they are few, or, where they are not cut and k is long, pairs with 128 rows, which fetch three quarters
-  // of the bytes (512 tokens, 11,008 x 4,096: 35 and 30 us).
+  // of the bytes (512 tokens, 11,008 x 4,096: 30.4 us, single blocks 29.9, which took 35 before their ring had six stages; 4,096 x 4,096: 14.7 and 13.7).
   const long long singles = (T + 127) / 128 * tiles_128, t_pairs = (T + 255) / 256;
   const long long waves_256 = (t_pairs * ((N + 255) / 256) * 2 + sms - 1) / sms, waves_128 = (t_pairs * ((N + 127) / 128) * 2 + sms - 1) / sms;
-  // Along k where that saves more than the joining takes (256 tokens, 4,096 x 4,096, 32 k blocks: 15.3 us uncut, 12.3 in two parts; 16 k blocks and 32 tiles:
-  // 8.1 us, 8.6 in four parts).
+  // Along k where that saves more than the joining takes (256 tokens, 4,096 x 4,096, 32 k blocks: 13.3 us uncut, 12.2 in two parts; 16 k blocks and 32 tiles:
+  // 8.2 us, 8.7 in four parts).
   a.cut = 1;
   if (a.blocks > 16)
     while (a.cut < 4 && singles * a.cut * 2 <= sms) a.cut *= 2;

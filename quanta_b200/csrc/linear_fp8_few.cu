@@ -13,9 +13,10 @@
 //   32           2,048 x 2,048 0.6 / 3.4 / 5.6, 4,096 x 2,048 1.3 / 5.2 / 7.0, 2,048 x 4,096 1.3 / 6.5 / 5.9, 4,096 x 4,096 2.6 / 10.7 / 8.2
 //   64           1,024 x 1,024 0.2 / 2.4 / 5.7, 2,048 x 2,048 0.6 / 6.4 / 6.6, 2,048 x 4,096 1.3 / 10.8 / 7.0
 //   128          1,024 x 1,024 0.2 / 4.3 / 6.0, 1,024 x 2,048 0.3 / 7.4 / 6.0;   256: 2,048 x 512 0.2 / 6.3 / 8.0;   1,000: 512 x 64 0 / 2.0 / 4.6
-// What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps and a cluster's parts before and behind the bytes; what bounds
-// this one in a large matrix or with many tokens is the issue of instructions (154 a warp for 2 KB and 8 tokens: e4m3 operands of mma.sync are converted
-// to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took the same time; four pieces ahead instead of two a
+// What tcgen05 takes more of a small matrix are the barriers, the tensor memory, the maps and a cluster's parts before and behind the bytes.  One token of a
+// large matrix is bound by the bytes, waves of blocks at a time: 4,096 x 9,472 (592 blocks, four an SM) 9.3 us, 18,944 16.0, 28,416 22.3, 37,888 28.3, 56,832 40.3,
+// so 3.1 us of start and end and 6.2 a full wave (38.8 MB, 0.96 of the rate of a copy); 22,016 is 2.3 waves and pays 1.2 us for the part (18.7).  With more
+// tokens it is the issue of instructions (154 a warp for 2 KB and 8 tokens: e4m3 operands of mma.sync are converted to fp16 first).  Blocks that walk over the rows, with the next rows' weights on their way, took the same time; four pieces ahead instead of two a
 // longer one in blocks of four warps (fewer of them).  Weights asked for before the launch ahead has ended (`early`): norm, product, activation and product of 4,096 x 11,008 for
 // one token 33.0 -> 32.2 us, for 32 38.1 -> 35.8, of 2,048 x 5,632 15.0 -> 13.7 and 22.5 -> 21.1.
 #include "fp8.cuh"
@@ -155,7 +156,7 @@ void l8f_launch(const LinearFp8Few& a, cudaStream_t stream) {
 
 // Whether products of T tokens and a [N, K] matrix are this kernel's.  Up to 8 tokens all but those of very many short rows; more as long as its
 // blocks are few for their length, blocks x (K + 4,096) at most 3 x 2^20, by the times above and those of some 200 sizes (K 256 to 11,008, N 512 to 10,000, 9 to 256
-// tokens), of which none is off by more than a tenth.
+// tokens), of which none is off by more than some tenth (32 tokens, 2,048 x 4,096, which lies on the line: 6.5 us, tcgen05 5.9).
 bool qb_linear_fp8_tokens_takes(int T, int K, int N) {
   if (T <= 8) return K >= 1024 || N <= 30000;
   const long long blocks = (long long)((N + 15) / 16) * ((T + 15) / 16);
