@@ -1256,6 +1256,13 @@ def glu_act(gate_up: torch.Tensor, out: torch.Tensor, *, bias=None, kind: int = 
                             ctypes.c_float(limit), ctypes.c_float(alpha), _stream()), "glu_act")
 
 
+def _want_status(status: torch.Tensor | None) -> None:
+    if status is not None:
+        _want(status, torch.int32, "status")
+        if status.numel() < 3:          # a kernel that has something to record writes three
+            raise ValueError(f"status must have the words of new_status, got {status.numel()}")
+
+
 FP8_BLOCK = 128                 # columns of a row, and rows and columns of a weight, that share a scale
 E4M3 = torch.float8_e4m3fn
 MOST_ROWS = 1 << 30             # rows, and columns of a row: the kernels count them, and what they take together, in 32 bits
@@ -1413,8 +1420,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError(f"linear_fp8: w_scales must be [{-(-N // FP8_BLOCK)}, {-(-K // FP8_BLOCK)}], got {tuple(w_scales.shape)}")
     if K == 0 or K % 16:
         raise ValueError(f"linear_fp8: K must be a positive multiple of 16, got {K}")
-    if status is not None:
-        _want(status, torch.int32, "status")
+    _want_status(status)
     device, (p_x, p_xs, p_w, p_ws, p_out, p_status) = _addresses(
         "linear_fp8", ("x", "x_scales", "w", "w_scales", "out", "status"), (x, x_scales, w, w_scales, out, status))
     fn = _entry("qb_linear_fp8", "pppppiiiiipp")
@@ -1458,8 +1464,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, logprob: t
             raise ValueError("token_logprobs: ids and best must be [n, k]")
         if top > min(V, TOKEN_LOGPROBS_MAX_TOP):
             raise ValueError(f"token_logprobs: {top} tokens a row of {V}; at most {TOKEN_LOGPROBS_MAX_TOP} are taken, and no more than there are")
-    if status is not None:
-        _want(status, torch.int32, "status")
+    _want_status(status)
     device, (p_x, p_t, p_lp, p_en, p_ids, p_best, p_status) = _addresses(
         "token_logprobs", ("logits", "tokens", "logprob", "entropy", "ids", "best", "status"),
         (logits, tokens, logprob, entropy, ids if top else None, best if top else None, status), strided=0)
