@@ -88,6 +88,12 @@ __device__ __forceinline__ float l8_remote(uint32_t addr) {
 
 constexpr int L8_NONE = 0x7fffffff;         // a NaN's bits
 
+// For a block that gave up: time (0.1 ms) for what it cannot wait on, copies or MMAs that are on their way
+__device__ __forceinline__ void l8_give_time() {
+  const uint64_t since = global_ns();
+  for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
+}
+
 // Eight parts of four neighbours, from the blocks of the cluster at this address, added in the order of the blocks.
 __device__ __forceinline__ float4 l8_sum_parts(uint32_t at, int cut) {
   float4 v[8];
@@ -204,8 +210,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       }
       if (*abort_flag && a.early && armed < min(a.stages, k_blocks)) {
         // weights are on their way whose tokens were not asked for, so that their barriers do not complete: give them time
-        const uint64_t since = global_ns();
-        for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
+        l8_give_time();
       }
       if (*abort_flag) {
         // let the copies that were issued land before this block's shared memory is given away
@@ -326,6 +331,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   // for may be of its own cluster, or of another that holds columns here and waits for them on another SM (at 64 tokens, 1,024 x 4,096, shared memory
   // places four blocks on an SM, tensor memory two).
   if (warp == 1) {
+    if (*abort_flag) l8_give_time();      // (MMAs whose accumulators nobody waited for)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM) : "memory");
   }
@@ -478,8 +484,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       const bool unarmed = !PAIR && a.early && armed < min(a.stages, k_blocks);
       if (*abort_flag && ((PAIR && rank != 0) || unarmed)) {
         // this block's copies count on the other block's barriers, which it cannot wait on, or on some that do not complete: give them time
-        const uint64_t since = global_ns();
-        for (uint32_t it = 0; it < TC_SPIN_LIMIT && global_ns() - since < 100000ull; ++it) __nanosleep(1000);
+        l8_give_time();
       } else if (*abort_flag) {
         // let the copies that were issued land before this block's shared memory is given away
         for (int i = max(0, armed - a.stages); i < armed; ++i) {
@@ -680,6 +685,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (warp == 1 && *abort_flag) l8_give_time();
   if constexpr (!PAIR) {      // before the cluster's barriers, as above
     if (warp == 1) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

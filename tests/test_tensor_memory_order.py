@@ -32,3 +32,12 @@ def test_tensor_memory_is_given_back_before_the_clusters_barriers(body):
 
 def test_the_kernels_are_found():
     assert len(list(_kernels())) >= 4
+
+
+def test_a_block_that_gave_up_gives_its_products_time():
+    """Nobody waits for the accumulators of a block that gave up, so it lets the products on their way end before the columns are another's."""
+    bodies = [b for n, _, b in _functions((build.SRC_DIR / "linear_fp8.cu").read_text()) if "tcgen05.dealloc" in b]
+    assert len(bodies) == 2
+    for body in bodies:
+        given = body.index("tcgen05.dealloc")
+        assert re.search(r"\*abort_flag\) l8_give_time\(\);", body[body.rindex("__syncthreads();", 0, given): given])
